@@ -293,6 +293,118 @@ int gdn_prefill_chunked_debug(const void *q, const void *k, const void *v, const
                               int64_t dbg_seq, int64_t dbg_head, int64_t dbg_chunk, void *stream);
 int64_t gdn_prefill_chunked_debug_floats(void);
 
+/* ------------------------------------------------------------------------- *
+ * Operators around the recurrence: the short convolution in front of a gated *
+ * delta rule or selective-scan layer, the selective scan, and the norm.  No  *
+ * counterpart in the reference, whose solutions stop at the delta rule.      *
+ * ------------------------------------------------------------------------- */
+
+/* Element type of the 16-bit tensors of gdn_conv, gdn_conv_pool and gdn_rms_norm. */
+enum gdn_dtype { GDN_BF16 = 0, GDN_F16 = 1 };
+
+/* gdn_conv / gdn_conv_pool flags */
+#define GDN_CONV_SILU 1              /* out = silu(sum), x * sigmoid(x) */
+
+/*
+ * Short causal depthwise convolution of packed prompts:
+ *   out[t, d] = act(bias[d] + sum_{j < width} weight[d, j] x~[t - width + 1 + j, d])
+ * with x~ before a sequence's first token taken from its state (the width - 1
+ * inputs before it, oldest first), or zero without one.
+ *
+ *   x         [T, dim], row t at x + t * x_row_stride elements
+ *   weight    [dim, width], bias [dim] or NULL
+ *   state     [N, width - 1, dim] or NULL     new_state [N, width - 1, dim]
+ *   cu_seqlens [N+1] int64, device memory, non-decreasing
+ *   outputs   num_outputs (1..4) host array of device pointers: contiguous
+ *             [T, widths[i]] tensors that take the channels in order (widths a host
+ *             array of multiples of 8 that sum to dim), e.g. q | k | v
+ * All tensors are of `dtype`; width is 2, 3 or 4; dim and x_row_stride are multiples
+ * of 8 and every buffer 16-byte aligned.  Sums are fp32, rounded once.  A sequence of
+ * length 0 keeps its state.  Rows of no sequence (before cu_seqlens[0] or from
+ * cu_seqlens[N] on) are left as they were.  new_state may not overlap state, and the
+ * outputs nothing else.  cu_seqlens is read only on the device, clamped to [0, T].
+ */
+int gdn_conv(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
+             const void *state, const int64_t *cu_seqlens, void *const *outputs,
+             const int64_t *widths, int num_outputs, void *new_state, int64_t total_seq_len,
+             int64_t num_seqs, int64_t dim, int64_t width, int dtype, int flags, void *stream);
+
+/*
+ * The same convolution for seq_len >= 1 tokens of each sequence of a decode batch over
+ * a pool of states, updated in place:
+ *   x         [B, seq_len, dim], token t of sequence i at
+ *             x + i * x_batch_stride + t * x_row_stride elements
+ *   state_pool [pool_size, width - 1, dim]; in_slots, out_slots as in gdn_decode_pool
+ *   outputs   [B, seq_len, widths[i]], contiguous
+ * Slots as for gdn_decode_pool: a negative or out-of-range read slot means a zero
+ * state, such a write slot no write; two sequences writing the same slot, or one
+ * reading a slot another writes, race.
+ */
+int gdn_conv_pool(const void *x, int64_t x_batch_stride, int64_t x_row_stride, const void *weight,
+                  const void *bias, void *state_pool, int64_t pool_size, const int32_t *in_slots,
+                  const int32_t *out_slots, void *const *outputs, const int64_t *widths,
+                  int num_outputs, int64_t batch_size, int64_t seq_len, int64_t dim, int64_t width,
+                  int dtype, int flags, void *stream);
+
+/*
+ * Selective state-space scan of packed prompts, one decay per head and token:
+ *   dt = softplus(a + dt_bias),  S <- exp(-exp(A_log) dt) S + (dt x) B^T,  y = S C + D x
+ *
+ *   x         [T, H, P] bf16               B, C     [T, G, Ns] bf16 (head h: group h / (H / G))
+ *   state     [N, H, P, Ns] fp32 or NULL   a        [T, H] bf16
+ *   A_log, dt_bias [H] fp32                D        [H] fp32 or NULL (no skip term)
+ *   cu_seqlens [N+1] int64, device         output   [T, H, P] bf16
+ *   new_state [N, H, P, Ns] fp32, may not overlap state
+ * P (head_dim) and Ns (state_dim) are 64 or 128; num_heads is a multiple of num_groups.
+ * The state is in the k-last layout of gdn_prefill.  A sequence of length 0 keeps its
+ * state.  Rows of no sequence are left as they were.  Buffers need 16-byte alignment.
+ * workspace: gdn_ssm_workspace_bytes bytes, 256-byte aligned (may be NULL when that
+ * is 0, and when NULL the call runs without cutting sequences).
+ */
+int gdn_ssm(const void *x, const void *B, const void *C, const float *state, const float *A_log,
+            const void *a, const float *dt_bias, const float *D, const int64_t *cu_seqlens,
+            void *output, float *new_state, int64_t total_seq_len, int64_t num_seqs,
+            int64_t num_heads, int64_t num_groups, int64_t head_dim, int64_t state_dim,
+            void *workspace, size_t workspace_bytes, void *stream);
+size_t gdn_ssm_workspace_bytes(int64_t total_seq_len, int64_t num_seqs, int64_t num_heads,
+                               int64_t num_groups, int64_t head_dim, int64_t state_dim);
+
+/*
+ * The same scan for seq_len >= 1 tokens of each sequence of a decode batch over a pool
+ * of states in fp32 or bf16 (enum gdn_state_dtype), updated in place unless flags has
+ * GDN_POOL_NO_STATE_UPDATE:
+ *   x [B, seq_len, H, P], B, C [B, seq_len, G, Ns], a [B, seq_len, H], output as x
+ *   state_pool [pool_size, H, P, Ns]; slots as in gdn_decode_pool
+ */
+int gdn_ssm_pool(const void *x, const void *B, const void *C, const float *A_log, const void *a,
+                 const float *dt_bias, const float *D, void *state_pool, int state_dtype,
+                 int64_t pool_size, const int32_t *in_slots, const int32_t *out_slots, int flags,
+                 void *output, int64_t batch_size, int64_t seq_len, int64_t num_heads,
+                 int64_t num_groups, int64_t head_dim, int64_t state_dim, void *stream);
+
+/* gdn_rms_norm flags */
+#define GDN_NORM_GATE_FIRST 1        /* norm(x silu(gate)) instead of norm(x) silu(gate) */
+
+/*
+ * Root-mean-square norm of rows:
+ *   h = x (+ residual) (* silu(gate) with GDN_NORM_GATE_FIRST)
+ *   y = h / sqrt(mean(h^2) + eps) * weight (* silu(gate) without it)
+ *
+ *   x, residual, gate  [rows, dim] of `dtype`, row r at + r * their row stride
+ *             (elements); residual or gate may be NULL, and not both given
+ *   weight    [dim]                 residual_out [rows, dim]: x + residual rounded once
+ *             (NULL without residual; may be residual itself when that is contiguous)
+ *   output    [rows, dim] of `dtype`, or with `scale` e4m3 (1 byte): y / scale with
+ *   scale     [rows] (group_size 0) or [rows, dim / 128] (group_size 128) fp32:
+ *             max |y| of the row or group / 448 (1 where that maximum is below 2^-100)
+ * y is fp32 up to the output's one rounding.  dim is a multiple of 8 (of 128 with
+ * group_size 128) up to 16384; strides are multiples of 8, buffers 16-byte aligned.
+ */
+int gdn_rms_norm(const void *x, int64_t x_row_stride, const void *weight, const void *residual,
+                 int64_t residual_row_stride, const void *gate, int64_t gate_row_stride, float eps,
+                 void *output, float *scale, int64_t group_size, void *residual_out, int64_t rows,
+                 int64_t dim, int dtype, int flags, void *stream);
+
 /*
  * Device status word.  A kernel that gives up on a bounded wait (an mbarrier
  * that does not complete within 2 s) sets a bit here and returns instead of

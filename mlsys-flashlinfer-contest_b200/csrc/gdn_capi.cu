@@ -408,4 +408,199 @@ int gdn_prep_meta(const int64_t* cu_seqlens, int64_t N, int32_t* chunk_offsets,
                      "gdn_prep_meta launch");
 }
 
+// Byte ranges [p, p + np) and [q, q + nq) share a byte.
+static bool overlap(const void* p, size_t np, const void* q, size_t nq) {
+  if (!p || !q || !np || !nq) return false;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + nq && b < a + np;
+}
+
+static int check_conv(const void* x, int64_t x_batch, int64_t x_row, const void* weight, const void* bias,
+                      void* const* outputs, const int64_t* widths, int count, int64_t T, int64_t N,
+                      int64_t D, int64_t W, int dtype, int flags, gdn::ConvArgs* a) {
+  if (W < 2 || W > 4) return fail(GDN_ERR_VALUE, "width must be 2, 3 or 4 (got %lld)", (long long)W);
+  if (D <= 0 || D % 8 != 0)
+    return fail(GDN_ERR_VALUE, "dim must be a positive multiple of 8 (got %lld)", (long long)D);
+  if (T < 0 || N < 0) return fail(GDN_ERR_VALUE, "lengths and counts must be non-negative");
+  if (dtype != GDN_BF16 && dtype != GDN_F16) return fail(GDN_ERR_TYPE, "dtype must be GDN_BF16 or GDN_F16");
+  if (flags & ~GDN_CONV_SILU) return fail(GDN_ERR_VALUE, "unknown flags");
+  if (count < 1 || count > gdn::kMaxConvOutputs)
+    return fail(GDN_ERR_VALUE, "num_outputs must be in [1, %d]", gdn::kMaxConvOutputs);
+  if (!weight || !outputs || !widths || (T > 0 && !x)) return fail(GDN_ERR_VALUE, "null pointer argument");
+  if (x_row < D || x_row % 8 != 0 || x_batch < 0 || x_batch % 8 != 0)
+    return fail(GDN_ERR_VALUE, "x strides must be multiples of 8 and rows at least dim apart");
+  if (!aligned(x, 16) || !aligned(weight, 16) || !aligned(bias, 16))
+    return fail(GDN_ERR_VALUE, "x, weight and bias must be 16-byte aligned");
+  int64_t sum = 0;
+  for (int i = 0; i < count; ++i) {
+    if (widths[i] <= 0 || widths[i] % 8 != 0)
+      return fail(GDN_ERR_VALUE, "output widths must be positive multiples of 8");
+    if ((T > 0 && !outputs[i]) || !aligned(outputs[i], 16))
+      return fail(GDN_ERR_VALUE, "output %d is null or not 16-byte aligned", i);
+    a->out.ptr[i] = outputs[i];
+    a->out.width[i] = widths[i];
+    sum += widths[i];
+  }
+  if (sum != D) return fail(GDN_ERR_VALUE, "output widths must sum to dim");
+  a->out.count = count;
+  a->x = x;
+  a->weight = weight;
+  a->bias = bias;
+  a->x_batch_stride = x_batch;
+  a->x_row_stride = x_row;
+  a->T = T;
+  a->N = N;
+  a->D = D;
+  a->W = W;
+  a->fp16 = dtype == GDN_F16;
+  a->silu = (flags & GDN_CONV_SILU) != 0;
+  return GDN_OK;
+}
+
+int gdn_conv(const void* x, int64_t x_row_stride, const void* weight, const void* bias, const void* state,
+             const int64_t* cu_seqlens, void* const* outputs, const int64_t* widths, int num_outputs,
+             void* new_state, int64_t T, int64_t N, int64_t D, int64_t W, int dtype, int flags,
+             void* stream) {
+  gdn::ConvArgs a{};
+  if (N <= 0) return fail(GDN_ERR_VALUE, "must have at least one sequence");
+  if (int e = check_conv(x, 0, x_row_stride, weight, bias, outputs, widths, num_outputs, T, N, D, W, dtype,
+                         flags, &a))
+    return e;
+  if (!cu_seqlens || !new_state) return fail(GDN_ERR_VALUE, "null pointer argument");
+  if (!aligned(state, 16) || !aligned(new_state, 16) || !aligned(cu_seqlens, 8))
+    return fail(GDN_ERR_VALUE, "state and new_state must be 16-byte and cu_seqlens 8-byte aligned");
+  const size_t bytes = static_cast<size_t>(N) * (W - 1) * D * 2;
+  if (overlap(state, bytes, new_state, bytes)) return fail(GDN_ERR_VALUE, "new_state overlaps state");
+  a.state = state;
+  a.new_state = new_state;
+  a.cu_seqlens = cu_seqlens;
+  return cuda_status(gdn::launch_conv(a, static_cast<cudaStream_t>(stream)), "gdn_conv launch");
+}
+
+int gdn_conv_pool(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const void* weight,
+                  const void* bias, void* state_pool, int64_t pool_size, const int32_t* in_slots,
+                  const int32_t* out_slots, void* const* outputs, const int64_t* widths, int num_outputs,
+                  int64_t B, int64_t T, int64_t D, int64_t W, int dtype, int flags, void* stream) {
+  gdn::ConvArgs a{};
+  if (B < 0) return fail(GDN_ERR_VALUE, "batch_size must be non-negative");
+  if (T < 1) return fail(GDN_ERR_VALUE, "seq_len must be at least 1");
+  if (pool_size < 0 || pool_size > INT32_MAX)
+    return fail(GDN_ERR_VALUE, "pool_size must be non-negative and fit int32 slot indices");
+  if (B == 0) return ok();
+  if (int e = check_conv(x, x_batch_stride, x_row_stride, weight, bias, outputs, widths, num_outputs, T, B,
+                         D, W, dtype, flags, &a))
+    return e;
+  if (!in_slots || (pool_size > 0 && !state_pool)) return fail(GDN_ERR_VALUE, "null pointer argument");
+  if (!aligned(state_pool, 16)) return fail(GDN_ERR_VALUE, "state_pool must be 16-byte aligned");
+  if (!aligned(in_slots, 4) || !aligned(out_slots, 4))
+    return fail(GDN_ERR_VALUE, "slot arrays must be 4-byte aligned");
+  a.pool = state_pool;
+  a.pool_size = pool_size;
+  a.in_slots = in_slots;
+  a.out_slots = out_slots;
+  return cuda_status(gdn::launch_conv(a, static_cast<cudaStream_t>(stream)), "gdn_conv_pool launch");
+}
+
+static int check_ssm(const void* x, const void* B, const void* C, const float* A_log, const void* a,
+                     const float* dt_bias, const void* y, int64_t T, int64_t H, int64_t G, int64_t P,
+                     int64_t Ns) {
+  if (H <= 0 || G <= 0 || H % G != 0)
+    return fail(GDN_ERR_VALUE, "num_heads (%lld) must be a positive multiple of num_groups (%lld)",
+                (long long)H, (long long)G);
+  if (P != 64 && P != 128) return fail(GDN_ERR_VALUE, "head_dim must be 64 or 128 (got %lld)", (long long)P);
+  if (Ns != 64 && Ns != 128)
+    return fail(GDN_ERR_VALUE, "state_dim must be 64 or 128 (got %lld)", (long long)Ns);
+  if (!A_log || !dt_bias || (T > 0 && (!x || !B || !C || !a || !y)))
+    return fail(GDN_ERR_VALUE, "null pointer argument");
+  if (!aligned(x, 16) || !aligned(B, 16) || !aligned(C, 16) || !aligned(y, 16) || !aligned(a, 2))
+    return fail(GDN_ERR_VALUE, "x, B, C and output must be 16-byte aligned");
+  return GDN_OK;
+}
+
+size_t gdn_ssm_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P, int64_t Ns) {
+  (void)T, (void)N, (void)H, (void)G, (void)P, (void)Ns;
+  return 0;
+}
+
+int gdn_ssm(const void* x, const void* B, const void* C, const float* state, const float* A_log,
+            const void* a, const float* dt_bias, const float* D, const int64_t* cu_seqlens, void* output,
+            float* new_state, int64_t T, int64_t N, int64_t H, int64_t G, int64_t P, int64_t Ns,
+            void* workspace, size_t workspace_bytes, void* stream) {
+  if (N <= 0) return fail(GDN_ERR_VALUE, "must have at least one sequence");
+  if (T < 0) return fail(GDN_ERR_VALUE, "total_seq_len must be non-negative");
+  if (int e = check_ssm(x, B, C, A_log, a, dt_bias, output, T, H, G, P, Ns)) return e;
+  if (!cu_seqlens || !new_state) return fail(GDN_ERR_VALUE, "null pointer argument");
+  if (!aligned(state, 16) || !aligned(new_state, 16) || !aligned(cu_seqlens, 8))
+    return fail(GDN_ERR_VALUE, "state and new_state must be 16-byte and cu_seqlens 8-byte aligned");
+  if (T > 0x7fffffffLL - 64) return fail(GDN_ERR_VALUE, "total_seq_len too large");
+  const size_t bytes = static_cast<size_t>(N) * H * P * Ns * 4;
+  if (overlap(state, bytes, new_state, bytes)) return fail(GDN_ERR_VALUE, "new_state overlaps state");
+  (void)workspace, (void)workspace_bytes;
+  gdn::SsmArgs p{};
+  p.x = x, p.B = B, p.C = C, p.state = state, p.A_log = A_log, p.a = a, p.dt_bias = dt_bias, p.D = D;
+  p.cu_seqlens = cu_seqlens, p.out = output, p.new_state = new_state;
+  p.T = T, p.N = N, p.H = H, p.G = G, p.P = P, p.Ns = Ns;
+  return cuda_status(gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream)), "gdn_ssm launch");
+}
+
+int gdn_ssm_pool(const void* x, const void* B, const void* C, const float* A_log, const void* a,
+                 const float* dt_bias, const float* D, void* state_pool, int state_dtype, int64_t pool_size,
+                 const int32_t* in_slots, const int32_t* out_slots, int flags, void* output, int64_t batch,
+                 int64_t T, int64_t H, int64_t G, int64_t P, int64_t Ns, void* stream) {
+  if (batch < 0) return fail(GDN_ERR_VALUE, "batch_size must be non-negative");
+  if (T < 1) return fail(GDN_ERR_VALUE, "seq_len must be at least 1");
+  if (pool_size < 0 || pool_size > INT32_MAX)
+    return fail(GDN_ERR_VALUE, "pool_size must be non-negative and fit int32 slot indices");
+  if (state_dtype != GDN_STATE_F32 && state_dtype != GDN_STATE_BF16)
+    return fail(GDN_ERR_TYPE, "state_dtype must be GDN_STATE_F32 or GDN_STATE_BF16");
+  if (flags & ~GDN_POOL_NO_STATE_UPDATE) return fail(GDN_ERR_VALUE, "unknown flags");
+  if (batch == 0) return ok();
+  if (int e = check_ssm(x, B, C, A_log, a, dt_bias, output, T, H, G, P, Ns)) return e;
+  if (!in_slots || (pool_size > 0 && !state_pool)) return fail(GDN_ERR_VALUE, "null pointer argument");
+  if (!aligned(state_pool, 16)) return fail(GDN_ERR_VALUE, "state_pool must be 16-byte aligned");
+  if (!aligned(in_slots, 4) || !aligned(out_slots, 4))
+    return fail(GDN_ERR_VALUE, "slot arrays must be 4-byte aligned");
+  gdn::SsmArgs p{};
+  p.x = x, p.B = B, p.C = C, p.A_log = A_log, p.a = a, p.dt_bias = dt_bias, p.D = D;
+  p.out = output, p.pool = state_pool, p.in_slots = in_slots, p.out_slots = out_slots;
+  p.T = T, p.N = batch, p.H = H, p.G = G, p.P = P, p.Ns = Ns, p.pool_size = pool_size;
+  p.state_bf16 = state_dtype == GDN_STATE_BF16;
+  p.no_state_update = (flags & GDN_POOL_NO_STATE_UPDATE) != 0;
+  return cuda_status(gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream)), "gdn_ssm_pool launch");
+}
+
+int gdn_rms_norm(const void* x, int64_t x_stride, const void* weight, const void* residual,
+                 int64_t residual_stride, const void* gate, int64_t gate_stride, float eps, void* output,
+                 float* scale, int64_t group, void* residual_out, int64_t rows, int64_t D, int dtype,
+                 int flags, void* stream) {
+  if (D <= 0 || D % 8 != 0 || D > 16384)
+    return fail(GDN_ERR_VALUE, "dim must be a multiple of 8 up to 16384 (got %lld)", (long long)D);
+  if (rows < 0) return fail(GDN_ERR_VALUE, "rows must be non-negative");
+  if (dtype != GDN_BF16 && dtype != GDN_F16) return fail(GDN_ERR_TYPE, "dtype must be GDN_BF16 or GDN_F16");
+  if (flags & ~GDN_NORM_GATE_FIRST) return fail(GDN_ERR_VALUE, "unknown flags");
+  if (group != 0 && (group != 128 || D % 128 != 0))
+    return fail(GDN_ERR_VALUE, "group_size must be 0, or 128 with dim a multiple of 128");
+  if (group != 0 && !scale) return fail(GDN_ERR_VALUE, "group_size needs a scale output");
+  if (residual && gate) return fail(GDN_ERR_VALUE, "residual and gate cannot both be given");
+  if ((residual != nullptr) != (residual_out != nullptr) && rows > 0)
+    return fail(GDN_ERR_VALUE, "residual_out goes with residual");
+  if (rows == 0) return ok();
+  if (!x || !weight || !output) return fail(GDN_ERR_VALUE, "null pointer argument");
+  if (!aligned(x, 16) || !aligned(weight, 16) || !aligned(residual, 16) || !aligned(gate, 16) ||
+      !aligned(output, 16) || !aligned(residual_out, 16) || !aligned(scale, 4))
+    return fail(GDN_ERR_VALUE, "buffers must be 16-byte aligned");
+  const int64_t strides[3] = {x_stride, residual ? residual_stride : D, gate ? gate_stride : D};
+  for (int64_t st : strides)
+    if (st < D || st % 8 != 0)
+      return fail(GDN_ERR_VALUE, "row strides must be multiples of 8 and at least dim");
+  const size_t span = (static_cast<size_t>(rows - 1) * (residual ? residual_stride : D) + D) * 2;
+  if (residual && overlap(residual, span, residual_out, static_cast<size_t>(rows) * D * 2) &&
+      !(residual == residual_out && residual_stride == D))
+    return fail(GDN_ERR_VALUE, "residual_out overlaps residual without being the same buffer");
+  const gdn::NormArgs a{x, weight, residual, gate, output, scale, residual_out, x_stride, residual_stride,
+                        gate_stride, rows, D, group, eps, dtype == GDN_F16,
+                        (flags & GDN_NORM_GATE_FIRST) != 0};
+  return cuda_status(gdn::launch_rms_norm(a, static_cast<cudaStream_t>(stream)), "gdn_rms_norm launch");
+}
+
 }  // extern "C"

@@ -139,6 +139,71 @@ cudaError_t launch_prefill_chunked_debug(const PrefillArgs& a, float* debug, int
                                          int dbg_head, int dbg_chunk, cudaStream_t s);
 int prefill_chunked_debug_floats();
 
+// Short causal depthwise convolution (gdn_conv.cu): packed prompts (cu_seqlens,
+// state -> new_state) or, with in_slots, T tokens of each of N sequences over a pool
+// of states updated in place.  Channels go to out.count contiguous tensors in order.
+constexpr int kMaxConvOutputs = 4;
+struct ConvOutputs {
+  void* ptr[kMaxConvOutputs];
+  int64_t width[kMaxConvOutputs];  // multiples of 8, summing to D
+  int count;
+};
+struct ConvArgs {
+  const void* x;        // rows of D 16-bit values: [T, D], or [N, T, D] with in_slots
+  const void* weight;   // [D, W]
+  const void* bias;     // [D] or nullptr
+  const void* state;    // [N, W-1, D] or nullptr (zero)
+  void* new_state;      // [N, W-1, D]
+  void* pool;           // [pool_size, W-1, D]
+  const int64_t* cu_seqlens;  // [N+1]
+  const int32_t* in_slots;    // [N] or nullptr (packed prompts)
+  const int32_t* out_slots;   // [N] or nullptr (= in_slots)
+  int64_t x_batch_stride, x_row_stride;  // in elements
+  int64_t T, N, D, W, pool_size;
+  bool fp16, silu;
+  ConvOutputs out;
+};
+cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s);
+
+// Selective state-space scan with one decay per head (gdn_ssm.cu, gdn_ssm_chunked.cu):
+// dt = softplus(a + dt_bias), S <- exp(-exp(A_log) dt) S + dt x B^T, y = S C + D x.
+struct SsmArgs {
+  const void* x;         // [T, H, P] bf16, or [N, T, H, P] with in_slots
+  const void* B;         // [T, G, Ns] bf16 ([N, T, G, Ns])
+  const void* C;         // as B
+  const float* state;    // [N, H, P, Ns] or nullptr (zero)
+  const float* A_log;    // [H]
+  const void* a;         // [T, H] bf16 ([N, T, H])
+  const float* dt_bias;  // [H]
+  const float* D;        // [H] or nullptr (no skip term)
+  const int64_t* cu_seqlens;  // [N+1] (packed prompts)
+  void* out;             // as x
+  float* new_state;      // [N, H, P, Ns]
+  void* pool;            // [pool_size, H, P, Ns] fp32 or bf16
+  const int32_t* in_slots;   // [N] or nullptr (packed prompts)
+  const int32_t* out_slots;  // [N] or nullptr (= in_slots)
+  int64_t T, N, H, G, P, Ns, pool_size;
+  bool state_bf16, no_state_update;
+};
+// Token by token on CUDA cores, the state in registers: the pool form and short prompts.
+cudaError_t launch_ssm_recurrent(const SsmArgs& a, cudaStream_t s);
+
+// Root-mean-square norm over rows (gdn_norm.cu).
+struct NormArgs {
+  const void* x;         // [rows, D] 16-bit
+  const void* weight;    // [D]
+  const void* residual;  // [rows, D] or nullptr
+  const void* gate;      // [rows, D] or nullptr
+  void* out;             // [rows, D]: the type of x, or e4m3 with `scale`
+  float* scale;          // [rows] or [rows, D / group], or nullptr
+  void* residual_out;    // [rows, D] with residual
+  int64_t x_stride, residual_stride, gate_stride;  // row strides in elements
+  int64_t rows, D, group;
+  float eps;
+  bool fp16, gate_first;
+};
+cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t s);
+
 // bounded wait on an mbarrier nothing arrives on (timeout path test)
 cudaError_t launch_wait_probe(uint64_t timeout_ns, uint32_t* result, cudaStream_t s);
 // device status word (bit flags of kernels that gave up on a wait)

@@ -1,0 +1,219 @@
+// Root-mean-square norm of rows with, optionally, the residual's addition in front, a
+// SiLU gate before or after, and an e4m3 output with fp32 scales (sm_100a).
+//
+//   h = x (+ residual; h rounded once is residual_out) (* silu(gate) with gate_first)
+//   y = h / sqrt(mean h^2 + eps) * weight (* silu(gate) without gate_first)
+//   e4m3: scale = max |y| / 448 over the row or over each 128 columns (1 where the
+//   maximum is 0 or below 2^-100), out = y / scale rounded to nearest (the quotient as
+//   a product with the rounded reciprocal: within 2 ulp of fp32).
+// h and y stay in fp32 from the loads to the one rounding of the output: the
+// quantised values come from y itself, not from a 16-bit y, and the norm from the
+// unrounded sum.
+//
+// Bound by HBM (one pass: every input is read once, kept in registers across the
+// reduction).  A row belongs to kLanes threads, each holding kVecs 16-byte pieces.
+#include "gdn_internal.h"
+#include "gdn_vec16.cuh"
+
+namespace gdn {
+namespace {
+
+constexpr float kE4m3Max = 448.0f;
+// Below this a row is all zero in e4m3 at scale 1, and its own scale (or the scale's
+// reciprocal) would leave fp32's normal range.
+constexpr float kTinyMax = 0x1p-100f;
+
+// The larger of the two, NaN if either is (a row that holds a NaN gets a NaN scale
+// instead of hiding it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+
+struct AddOp {
+  static __device__ __forceinline__ float f(float a, float b) { return a + b; }
+};
+struct MaxOp {
+  static __device__ __forceinline__ float f(float a, float b) { return max_nan(a, b); }
+};
+
+// Reduction over the kLanes threads of a row (every thread gets the result).  Rows of
+// more than a warp go through shared memory; `slot` is a buffer no earlier reduction
+// of this block used.
+template <class Op, int kLanes>
+__device__ __forceinline__ float row_reduce(float v, float* slot) {
+#pragma unroll
+  for (int d = 1; d < (kLanes < 32 ? kLanes : 32); d <<= 1)
+    v = Op::f(v, __shfl_xor_sync(0xffffffffu, v, d));
+  if constexpr (kLanes > 32) {
+    constexpr int kWarps = kLanes / 32;
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) slot[warp] = v;
+    __syncthreads();
+    const float* mine = slot + warp / kWarps * kWarps;
+    v = mine[0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) v = Op::f(v, mine[i]);
+  }
+  return v;
+}
+
+enum GateMode { kNoGate = 0, kGateAfter = 1, kGateFirst = 2 };
+
+template <class T, int kLanes, int kVecs, int kThreads, bool RESIDUAL, int GATE, bool FP8>
+__global__ void __launch_bounds__(kThreads) gdn_rms_norm_kernel(NormArgs p) {
+  constexpr int kRows = kThreads / kLanes;
+  __shared__ float slots[2][kThreads / 32];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const bool live = row < p.rows;
+  const int nvec = static_cast<int>(p.D >> 3);
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.x_stride;
+  const uint16_t* res = static_cast<const uint16_t*>(p.residual) + row * p.residual_stride;
+  const uint16_t* gate = static_cast<const uint16_t*>(p.gate) + row * p.gate_stride;
+  const uint16_t* weight = static_cast<const uint16_t*>(p.weight);
+
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 xr[kVecs], rr[kVecs], gr[kVecs], wr[kVecs];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int i = lane + k * kLanes;
+    const bool in = live && i < nvec;
+    xr[k] = in ? ld_cs_u4(x + 8 * i) : zero;
+    if (RESIDUAL) rr[k] = in ? ld_cs_u4(res + 8 * i) : zero;
+    if (GATE != kNoGate) gr[k] = in ? ld_cs_u4(gate + 8 * i) : zero;
+  }
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int i = lane + k * kLanes;
+    wr[k] = i < nvec ? ldg_u4(weight + 8 * i) : zero;
+  }
+
+  float h[kVecs][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    unpack8<T>(xr[k], h[k]);
+    if (RESIDUAL) {
+      float r[8];
+      unpack8<T>(rr[k], r);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[k][e] += r[e];
+      const int i = lane + k * kLanes;
+      if (live && i < nvec)
+        st_u4(static_cast<uint16_t*>(p.residual_out) + row * p.D + 8 * i, pack8<T>(h[k]));
+    }
+    if (GATE == kGateFirst) {
+      float g[8];
+      unpack8<T>(gr[k], g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[k][e] *= silu(g[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(h[k][e], h[k][e], ss);
+  }
+  ss = row_reduce<AddOp, kLanes>(ss, slots[0]);
+  const float inv = 1.0f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
+
+  float amax = 0.f;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    float w[8];
+    unpack8<T>(wr[k], w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[k][e] *= inv * w[e];
+    if (GATE == kGateAfter) {
+      float g[8];
+      unpack8<T>(gr[k], g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[k][e] *= silu(g[e]);
+    }
+    if constexpr (!FP8) {
+      const int i = lane + k * kLanes;
+      if (live && i < nvec) st_u4(static_cast<uint16_t*>(p.out) + row * p.D + 8 * i, pack8<T>(h[k]));
+    } else if (p.group == 0) {
+      // (lanes past the row hold weight 0 and h 0, but 0 * inv is NaN where inv is not
+      // finite; such a row is NaN anyway)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(h[k][e]));
+    }
+  }
+  if constexpr (FP8) {
+    if (p.group == 0) amax = row_reduce<MaxOp, kLanes>(amax, slots[1]);
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int i = lane + k * kLanes;
+      if (p.group != 0) {  // 128 columns = 16 neighbouring lanes
+        amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(h[k][e]));
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+      }
+      // (a NaN maximum fails the comparison and stays)
+      const float scale = amax < kTinyMax ? 1.f : amax / kE4m3Max;
+      const float rs = 1.f / scale;
+      if (live && i < nvec) {
+        if (p.group != 0) {
+          if ((i & 15) == 0) p.scale[row * (p.D >> 7) + (i >> 4)] = scale;
+        } else if (i == 0) {
+          p.scale[row] = scale;
+        }
+        uint2 q;
+        q.x = e4m3x4(h[k][0] * rs, h[k][1] * rs, h[k][2] * rs, h[k][3] * rs);
+        q.y = e4m3x4(h[k][4] * rs, h[k][5] * rs, h[k][6] * rs, h[k][7] * rs);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + row * p.D + 8 * i) = q;
+      }
+    }
+  }
+}
+
+template <class T, int kLanes, int kVecs, int kThreads>
+cudaError_t launch(const NormArgs& a, cudaStream_t s) {
+  constexpr int kRows = kThreads / kLanes;
+  const int64_t blocks = (a.rows + kRows - 1) / kRows;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const unsigned g = static_cast<unsigned>(blocks);
+  const bool fp8 = a.scale != nullptr;
+  const int gate = !a.gate ? kNoGate : a.gate_first ? kGateFirst : kGateAfter;
+#define GDN_NORM(R, GATE, Q) gdn_rms_norm_kernel<T, kLanes, kVecs, kThreads, R, GATE, Q><<<g, kThreads, 0, s>>>(a)
+  if (a.residual)
+    fp8 ? GDN_NORM(true, kNoGate, true) : GDN_NORM(true, kNoGate, false);
+  else if (gate == kGateFirst)
+    fp8 ? GDN_NORM(false, kGateFirst, true) : GDN_NORM(false, kGateFirst, false);
+  else if (gate == kGateAfter)
+    fp8 ? GDN_NORM(false, kGateAfter, true) : GDN_NORM(false, kGateAfter, false);
+  else
+    fp8 ? GDN_NORM(false, kNoGate, true) : GDN_NORM(false, kNoGate, false);
+#undef GDN_NORM
+  return cudaGetLastError();
+}
+
+// Threads per row: a row's 16-byte pieces, at most four a thread.
+template <class T>
+cudaError_t by_size(const NormArgs& a, cudaStream_t s) {
+  const int64_t v = a.D / 8;
+  if (v <= 16) return launch<T, 16, 1, 256>(a, s);
+  if (v <= 32) return launch<T, 32, 1, 256>(a, s);
+  if (v <= 128) return launch<T, 128, 1, 128>(a, s);
+  if (v <= 256) return launch<T, 256, 1, 256>(a, s);
+  if (v <= 512) return launch<T, 256, 2, 256>(a, s);
+  if (v <= 1024) return launch<T, 512, 2, 512>(a, s);
+  return launch<T, 512, 4, 512>(a, s);
+}
+
+}  // namespace
+
+cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t s) {
+  return a.fp16 ? by_size<Fp16>(a, s) : by_size<Bf16>(a, s);
+}
+
+}  // namespace gdn

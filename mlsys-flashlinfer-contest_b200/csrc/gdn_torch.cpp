@@ -25,7 +25,9 @@ void cuda_contig(const at::Tensor& t, const char* name) {
 }
 
 void rank(const at::Tensor& t, const char* name, int64_t d) {
-  TORCH_CHECK_VALUE(t.dim() == d, name, " must be a ", d, "D tensor");
+  // (numbers go into messages through std::to_string: inserting them into the message's
+  // stream crashes in a process that has loaded the CUDA libraries)
+  TORCH_CHECK_VALUE(t.dim() == d, name, " must be a ", std::to_string(d), "D tensor");
 }
 
 void dtype(const at::Tensor& t, const char* name, at::ScalarType s) {
@@ -323,6 +325,298 @@ at::Tensor decode_pool(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   return *output;
 }
 
+// ---- convolution, selective scan, norm ----------------------------------------
+
+using OptTensor = c10::optional<at::Tensor>;
+
+void on_device(const at::Tensor& ref, const at::Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK_VALUE(t.device() == ref.device(), "x and ", name, " must be on the same device");
+}
+
+std::string shape_text(at::IntArrayRef s) {
+  std::string r = "[";
+  for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
+  return r + "]";
+}
+
+// contiguous, of x's device, the given type and shape
+void expect(const at::Tensor& ref, const at::Tensor& t, const char* name, at::ScalarType s,
+            at::IntArrayRef shape) {
+  on_device(ref, t, name);
+  TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK_TYPE(t.scalar_type() == s, name, " must be ", c10::toString(s), ", got ",
+                   c10::toString(t.scalar_type()));
+  TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape_text(shape), ", got ", shape_text(t.sizes()));
+}
+
+int dtype16(const at::Tensor& x) {
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+                   "x must be bfloat16 or float16");
+  return x.scalar_type() == at::kHalf ? GDN_F16 : GDN_BF16;
+}
+
+const void* opt_ptr(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+cudaStream_t stream_of(const at::Tensor& x) {
+  return c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+}
+
+// The output tensors of a convolution: leading sizes `lead`, widths `splits` (empty:
+// one output of all the channels), allocated unless given.
+std::vector<at::Tensor> conv_outputs(const at::Tensor& x, std::vector<int64_t>& splits,
+                                     c10::optional<std::vector<at::Tensor>>& given,
+                                     std::vector<void*>& ptrs) {
+  const int64_t D = x.size(-1);
+  if (splits.empty()) splits.push_back(D);
+  TORCH_CHECK_VALUE(splits.size() <= 4, "at most 4 splits");
+  int64_t sum = 0;
+  for (int64_t w : splits) {
+    TORCH_CHECK_VALUE(w > 0 && w % 8 == 0, "splits must be positive multiples of 8");
+    sum += w;
+  }
+  TORCH_CHECK_VALUE(sum == D, "splits must sum to the channels of x");
+  if (given.has_value())
+    TORCH_CHECK_VALUE(given->size() == splits.size(), "outputs must hold one tensor per split");
+  std::vector<at::Tensor> outs;
+  for (size_t i = 0; i < splits.size(); ++i) {
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = splits[i];
+    if (given.has_value()) {
+      expect(x, (*given)[i], "outputs", x.scalar_type(), shape);
+      outs.push_back((*given)[i]);
+    } else {
+      outs.push_back(at::empty(shape, x.options()));
+    }
+    ptrs.push_back(outs.back().data_ptr());
+  }
+  return outs;
+}
+
+int64_t conv_weights(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias) {
+  const int64_t D = x.size(-1);
+  rank(weight, "weight", 2);
+  const int64_t W = weight.size(1);
+  TORCH_CHECK_VALUE(W >= 2 && W <= 4, "the convolution's width must be 2, 3 or 4");
+  TORCH_CHECK_VALUE(D > 0 && D % 8 == 0, "the channels of x must be a positive multiple of 8");
+  expect(x, weight, "weight", x.scalar_type(), {D, W});
+  if (bias.has_value()) expect(x, *bias, "bias", x.scalar_type(), {D});
+  TORCH_CHECK_VALUE(x.stride(-1) == 1, "the channels of x must be contiguous");
+  return W;
+}
+
+// conv: x [T, D] (rows may be strided), weight [D, W], bias [D] or None, state
+// [N, W-1, D] or None, cu_seqlens [N+1] int64 -> ([outputs], new_state)
+std::tuple<std::vector<at::Tensor>, at::Tensor> conv(
+    const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias, const OptTensor& state,
+    const at::Tensor& cu_seqlens, bool silu, std::vector<int64_t> splits,
+    c10::optional<std::vector<at::Tensor>> outputs, OptTensor new_state) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
+  rank(x, "x", 2);
+  const int dt = dtype16(x);
+  const int64_t T = x.size(0), D = x.size(1), W = conv_weights(x, weight, bias);
+  rank(cu_seqlens, "cu_seqlens", 1);
+  const int64_t N = cu_seqlens.size(0) - 1;
+  TORCH_CHECK_VALUE(N > 0, "must have at least one sequence");
+  expect(x, cu_seqlens, "cu_seqlens", at::kLong, {N + 1});
+  if (state.has_value()) expect(x, *state, "state", x.scalar_type(), {N, W - 1, D});
+  if (new_state.has_value())
+    expect(x, *new_state, "new_state", x.scalar_type(), {N, W - 1, D});
+  else
+    new_state = at::empty({N, W - 1, D}, x.options());
+  std::vector<void*> ptrs;
+  std::vector<at::Tensor> outs = conv_outputs(x, splits, outputs, ptrs);
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(gdn_conv(x.data_ptr(), T > 1 ? x.stride(0) : D, weight.data_ptr(), opt_ptr(bias), opt_ptr(state),
+                    cu_seqlens.data_ptr<int64_t>(), ptrs.data(), splits.data(),
+                    static_cast<int>(splits.size()), new_state->data_ptr(), T, N, D, W, dt,
+                    silu ? GDN_CONV_SILU : 0, stream_of(x)),
+           "gdn_conv");
+  return {outs, *new_state};
+}
+
+// conv_pool: x [B, T, D] (batch and token strides), state_pool [P, W-1, D] (in place),
+// in_slots / out_slots [B] int32 -> [outputs]
+std::vector<at::Tensor> conv_pool(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                                  const at::Tensor& state_pool, const at::Tensor& in_slots,
+                                  const OptTensor& out_slots, bool silu, std::vector<int64_t> splits,
+                                  c10::optional<std::vector<at::Tensor>> outputs) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
+  rank(x, "x", 3);
+  const int dt = dtype16(x);
+  const int64_t B = x.size(0), T = x.size(1), D = x.size(2), W = conv_weights(x, weight, bias);
+  TORCH_CHECK_VALUE(T >= 1, "need at least one token per sequence");
+  rank(state_pool, "state_pool", 3);
+  expect(x, state_pool, "state_pool", x.scalar_type(), {state_pool.size(0), W - 1, D});
+  expect(x, in_slots, "in_slots", at::kInt, {B});
+  if (out_slots.has_value()) expect(x, *out_slots, "out_slots", at::kInt, {B});
+  std::vector<void*> ptrs;
+  std::vector<at::Tensor> outs = conv_outputs(x, splits, outputs, ptrs);
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(gdn_conv_pool(x.data_ptr(), B > 1 ? x.stride(0) : 0, T > 1 ? x.stride(1) : D, weight.data_ptr(),
+                         opt_ptr(bias), state_pool.data_ptr(), state_pool.size(0),
+                         in_slots.data_ptr<int32_t>(),
+                         out_slots.has_value() ? out_slots->data_ptr<int32_t>() : nullptr, ptrs.data(),
+                         splits.data(), static_cast<int>(splits.size()), B, T, D, W, dt,
+                         silu ? GDN_CONV_SILU : 0, stream_of(x)),
+           "gdn_conv_pool");
+  return outs;
+}
+
+struct SsmSizes {
+  int64_t H, P, G, Ns;
+};
+
+// The inputs of a scan whose tensors have the leading sizes `lead`.
+SsmSizes ssm_inputs(const at::Tensor& x, const at::Tensor& B, const at::Tensor& C, const at::Tensor& A_log,
+                    const at::Tensor& a, const at::Tensor& dt_bias, const OptTensor& D, int64_t nlead) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
+  rank(x, "x", nlead + 2);
+  rank(B, "B", nlead + 2);
+  const SsmSizes z{x.size(nlead), x.size(nlead + 1), B.size(nlead), B.size(nlead + 1)};
+  TORCH_CHECK_VALUE(z.H > 0 && z.G > 0 && z.H % z.G == 0, "the heads of x must be a positive multiple of B's groups");
+  TORCH_CHECK_VALUE(z.P == 64 || z.P == 128, "the head size of x must be 64 or 128");
+  TORCH_CHECK_VALUE(z.Ns == 64 || z.Ns == 128, "the state size of B and C must be 64 or 128");
+  std::vector<int64_t> xs(x.sizes().begin(), x.sizes().end()), bs = xs, as = xs;
+  bs[nlead] = z.G;
+  bs[nlead + 1] = z.Ns;
+  as.pop_back();
+  expect(x, x, "x", at::kBFloat16, xs);
+  expect(x, B, "B", at::kBFloat16, bs);
+  expect(x, C, "C", at::kBFloat16, bs);
+  expect(x, a, "a", at::kBFloat16, as);
+  expect(x, A_log, "A_log", at::kFloat, {z.H});
+  expect(x, dt_bias, "dt_bias", at::kFloat, {z.H});
+  if (D.has_value()) expect(x, *D, "D", at::kFloat, {z.H});
+  return z;
+}
+
+// ssm: x [T, H, P], B, C [T, G, Ns], a [T, H] bf16; state [N, H, P, Ns] fp32 or None;
+// cu_seqlens [N+1] int64 -> (output, new_state).  The workspace comes from the
+// caching allocator.
+std::tuple<at::Tensor, at::Tensor> ssm(const at::Tensor& x, const at::Tensor& B, const at::Tensor& C,
+                                       const OptTensor& state, const at::Tensor& A_log, const at::Tensor& a,
+                                       const at::Tensor& dt_bias, const OptTensor& D,
+                                       const at::Tensor& cu_seqlens, OptTensor output, OptTensor new_state) {
+  const SsmSizes z = ssm_inputs(x, B, C, A_log, a, dt_bias, D, 1);
+  const int64_t T = x.size(0);
+  rank(cu_seqlens, "cu_seqlens", 1);
+  const int64_t N = cu_seqlens.size(0) - 1;
+  TORCH_CHECK_VALUE(N > 0, "must have at least one sequence");
+  expect(x, cu_seqlens, "cu_seqlens", at::kLong, {N + 1});
+  const std::vector<int64_t> ss{N, z.H, z.P, z.Ns};
+  if (state.has_value()) expect(x, *state, "state", at::kFloat, ss);
+  if (output.has_value())
+    expect(x, *output, "output", at::kBFloat16, x.sizes());
+  else
+    output = at::empty(x.sizes(), x.options());
+  if (new_state.has_value())
+    expect(x, *new_state, "new_state", at::kFloat, ss);
+  else
+    new_state = at::empty(ss, x.options().dtype(at::kFloat));
+  const c10::cuda::CUDAGuard guard(x.device());
+  const size_t ws_bytes = gdn_ssm_workspace_bytes(T, N, z.H, z.G, z.P, z.Ns);
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
+  check_rc(gdn_ssm(x.data_ptr(), B.data_ptr(), C.data_ptr(), state_ptr(state), A_log.data_ptr<float>(),
+                   a.data_ptr(), dt_bias.data_ptr<float>(), state_ptr(D), cu_seqlens.data_ptr<int64_t>(),
+                   output->data_ptr(), new_state->data_ptr<float>(), T, N, z.H, z.G, z.P, z.Ns,
+                   ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, stream_of(x)),
+           "gdn_ssm");
+  return {*output, *new_state};
+}
+
+// ssm_pool: x [B, T, H, P], B, C [B, T, G, Ns], a [B, T, H] bf16; state_pool
+// [pool, H, P, Ns] fp32 or bf16 (in place); in_slots / out_slots [B] int32 -> output
+at::Tensor ssm_pool(const at::Tensor& x, const at::Tensor& B, const at::Tensor& C, const at::Tensor& A_log,
+                    const at::Tensor& a, const at::Tensor& dt_bias, const OptTensor& D,
+                    const at::Tensor& state_pool, const at::Tensor& in_slots, const OptTensor& out_slots,
+                    bool no_state_update, OptTensor output) {
+  const SsmSizes z = ssm_inputs(x, B, C, A_log, a, dt_bias, D, 2);
+  const int64_t batch = x.size(0), T = x.size(1);
+  TORCH_CHECK_VALUE(T >= 1, "need at least one token per sequence");
+  TORCH_CHECK_TYPE(state_pool.scalar_type() == at::kFloat || state_pool.scalar_type() == at::kBFloat16,
+                   "state_pool must be float32 or bfloat16");
+  rank(state_pool, "state_pool", 4);
+  expect(x, state_pool, "state_pool", state_pool.scalar_type(), {state_pool.size(0), z.H, z.P, z.Ns});
+  expect(x, in_slots, "in_slots", at::kInt, {batch});
+  if (out_slots.has_value()) expect(x, *out_slots, "out_slots", at::kInt, {batch});
+  if (output.has_value())
+    expect(x, *output, "output", at::kBFloat16, x.sizes());
+  else
+    output = at::empty(x.sizes(), x.options());
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(gdn_ssm_pool(x.data_ptr(), B.data_ptr(), C.data_ptr(), A_log.data_ptr<float>(), a.data_ptr(),
+                        dt_bias.data_ptr<float>(), state_ptr(D), state_pool.data_ptr(),
+                        state_pool.scalar_type() == at::kBFloat16 ? GDN_STATE_BF16 : GDN_STATE_F32,
+                        state_pool.size(0), in_slots.data_ptr<int32_t>(),
+                        out_slots.has_value() ? out_slots->data_ptr<int32_t>() : nullptr,
+                        no_state_update ? GDN_POOL_NO_STATE_UPDATE : 0, output->data_ptr(), batch, T, z.H,
+                        z.G, z.P, z.Ns, stream_of(x)),
+           "gdn_ssm_pool");
+  return *output;
+}
+
+// rms_norm: x [..., D] contiguous, or [rows, D] with a row stride (residual and gate
+// likewise, of x's shape); weight [D] -> [output (, scale) (, residual_out)].
+// fp8: e4m3 with scales by row (group 0) or by 128 columns (group 128).
+std::vector<at::Tensor> rms_norm(const at::Tensor& x, const at::Tensor& weight, double eps,
+                                 const OptTensor& residual, const OptTensor& gate, bool gate_first, bool fp8,
+                                 int64_t group, OptTensor output, OptTensor residual_out) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK_VALUE(x.dim() >= 1, "x must have at least one dimension");
+  const int dt = dtype16(x);
+  const int64_t D = x.size(-1);
+  TORCH_CHECK_VALUE(D > 0 && D % 8 == 0 && D <= 16384, "the rows of x must hold a multiple of 8 values, at most 16384");
+  TORCH_CHECK_VALUE(!(residual.has_value() && gate.has_value()), "residual and gate cannot both be given");
+  TORCH_CHECK_VALUE(residual.has_value() || !residual_out.has_value(), "residual_out goes with residual");
+  TORCH_CHECK_VALUE(group == 0 || (group == 128 && D % 128 == 0),
+                    "group_size must be 0, or 128 with rows of a multiple of 128");
+  const int64_t rows = x.numel() / D;
+  auto row_stride = [&](const at::Tensor& t, const char* name) -> int64_t {
+    on_device(x, t, name);
+    TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name, " must have the type of x");
+    TORCH_CHECK_VALUE(t.sizes() == x.sizes(), name, " must have the shape of x");
+    if (t.is_contiguous()) return D;
+    TORCH_CHECK_VALUE(t.dim() == 2 && t.stride(1) == 1, name, " must be contiguous, or 2D with contiguous rows");
+    return rows > 1 ? t.stride(0) : D;
+  };
+  const int64_t xs = row_stride(x, "x");
+  const int64_t rs = residual.has_value() ? row_stride(*residual, "residual") : D;
+  const int64_t gs = gate.has_value() ? row_stride(*gate, "gate") : D;
+  expect(x, weight, "weight", x.scalar_type(), {D});
+  const at::ScalarType ot = fp8 ? at::kFloat8_e4m3fn : x.scalar_type();
+  std::vector<at::Tensor> ret;
+  if (output.has_value())
+    expect(x, *output, "output", ot, x.sizes());
+  else
+    output = at::empty(x.sizes(), x.options().dtype(ot));
+  ret.push_back(*output);
+  if (fp8) {
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    if (group)
+      shape.back() = D / group;
+    else
+      shape.pop_back();
+    ret.push_back(at::empty(shape, x.options().dtype(at::kFloat)));
+  }
+  float* scale = fp8 ? ret.back().data_ptr<float>() : nullptr;
+  if (residual.has_value()) {
+    if (residual_out.has_value())
+      expect(x, *residual_out, "residual_out", x.scalar_type(), x.sizes());
+    else
+      residual_out = at::empty(x.sizes(), x.options());
+    ret.push_back(*residual_out);
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(gdn_rms_norm(x.data_ptr(), xs, weight.data_ptr(), opt_ptr(residual), rs, opt_ptr(gate), gs,
+                        static_cast<float>(eps), output->data_ptr(), scale, group,
+                        residual_out.has_value() ? residual_out->data_ptr() : nullptr, rows, D, dt,
+                        gate_first ? GDN_NORM_GATE_FIRST : 0, stream_of(x)),
+           "gdn_rms_norm");
+  return ret;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -342,4 +636,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out_slots") = py::none(), py::arg("intermediate") = py::none(),
         py::arg("qk_l2norm") = false, py::arg("no_state_update") = false,
         py::arg("output") = py::none());
+  m.def("conv", &conv, "short causal convolution of packed prompts (C ABI gdn_conv)", py::arg("x"),
+        py::arg("weight"), py::arg("bias"), py::arg("state"), py::arg("cu_seqlens"), py::arg("silu"),
+        py::arg("splits"), py::arg("outputs") = py::none(), py::arg("new_state") = py::none());
+  m.def("conv_pool", &conv_pool, "short causal convolution over a pool of states (C ABI gdn_conv_pool)",
+        py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("state_pool"), py::arg("in_slots"),
+        py::arg("out_slots"), py::arg("silu"), py::arg("splits"), py::arg("outputs") = py::none());
+  m.def("ssm", &ssm, "selective scan of packed prompts (C ABI gdn_ssm)", py::arg("x"), py::arg("B"),
+        py::arg("C"), py::arg("state"), py::arg("A_log"), py::arg("a"), py::arg("dt_bias"), py::arg("D"),
+        py::arg("cu_seqlens"), py::arg("output") = py::none(), py::arg("new_state") = py::none());
+  m.def("ssm_pool", &ssm_pool, "selective scan over a pool of states (C ABI gdn_ssm_pool)", py::arg("x"),
+        py::arg("B"), py::arg("C"), py::arg("A_log"), py::arg("a"), py::arg("dt_bias"), py::arg("D"),
+        py::arg("state_pool"), py::arg("in_slots"), py::arg("out_slots"), py::arg("no_state_update"),
+        py::arg("output") = py::none());
+  m.def("rms_norm", &rms_norm, "root-mean-square norm of rows (C ABI gdn_rms_norm)", py::arg("x"),
+        py::arg("weight"), py::arg("eps"), py::arg("residual"), py::arg("gate"), py::arg("gate_first"),
+        py::arg("fp8"), py::arg("group"), py::arg("output") = py::none(),
+        py::arg("residual_out") = py::none());
 }

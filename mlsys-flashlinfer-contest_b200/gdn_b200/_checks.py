@@ -40,3 +40,24 @@ def resolve_scale(scale) -> float:
     if isinstance(scale, torch.Tensor):
         scale = float(scale.item())
     return float(scale)
+
+
+def expect(ref, name, t, dt, shape):
+    """A contiguous CUDA tensor on ``ref``'s device, of the given dtype and shape."""
+    cuda_contig(name, t)
+    if t.device != ref.device:
+        raise ValueError(f"x and {name} must be on the same device")
+    dtype(name, t, dt)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def dtype16(t) -> int:
+    """The C ABI's enum gdn_dtype of a 16-bit CUDA tensor."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    if t.device.type != "cuda":
+        raise ValueError("x must be a CUDA tensor")
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("x must be bfloat16 or float16")
+    return int(t.dtype == torch.float16)

@@ -41,6 +41,12 @@ SIGNATURES = {
     "gdn_prefill_chunked_debug": (I, [P, P, P, P, P, P, P, P, P, F, P, P, I64, I64, I64, I64, I64,
                                       I64, P, I64, I64, I64, I64, P]),
     "gdn_prefill_chunked_debug_floats": (I64, []),
+    "gdn_conv": (I, [P, I64, P, P, P, P, P, P, I, P, I64, I64, I64, I64, I, I, P]),
+    "gdn_conv_pool": (I, [P, I64, I64, P, P, P, I64, P, P, P, P, I, I64, I64, I64, I64, I, I, P]),
+    "gdn_ssm": (I, [P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, SZ, P]),
+    "gdn_ssm_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I64]),
+    "gdn_ssm_pool": (I, [P, P, P, P, P, P, P, P, I, I64, P, P, I, P, I64, I64, I64, I64, I64, I64, P]),
+    "gdn_rms_norm": (I, [P, I64, P, P, I64, P, I64, F, P, P, I64, P, I64, I64, I, I, P]),
     "gdn_read_status": (I, [P, I]),
     "gdn_wait_probe": (I, [ctypes.c_uint64, P, P]),
 }

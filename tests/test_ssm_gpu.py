@@ -1,0 +1,174 @@
+"""The selective scan against its 64-bit definition (GPU)."""
+import pytest
+import torch
+
+import layer_oracle as L
+
+pytestmark = pytest.mark.gpu
+
+
+def make(lead, H, P, G, Ns, seed=0, skip=True):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*lead, *s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    A_log, dt_bias = L.gates(H, "cuda", g)
+    return dict(x=r(H, P), B=r(G, Ns), C=r(G, Ns), A_log=A_log, a=r(H), dt_bias=dt_bias,
+                D=torch.rand(H, generator=g, device="cuda") if skip else None)
+
+
+# Bounds.  fp32 arithmetic on a state that t tokens went into: every token multiplies it by a
+# decay whose relative error is a few 2^-24 (its exponent rounded, expf) and adds a product
+# of dt (log1pf, expf: a few 2^-24) -- 8 2^-24 a token, and 200 2^-24 for the rest, times
+# the magnitude.  Matrix products over chunks round two operands to bf16, the weights within the
+# chunk and the state that C reads (half a step, 2^-8, of each term), and split the
+# state's update into two bf16 terms (2^-8 of 2^-8).
+def y_slack(ya, n):
+    return (2.0 ** -8 + (8 * n + 200) * 2.0 ** -24) * ya
+
+
+def s_slack(Sa, n):
+    return (2.0 ** -16 + (8 * n + 200) * 2.0 ** -24) * Sa
+
+
+def f32_slack(mag, n):
+    return (8 * n + 200) * 2.0 ** -24 * mag
+
+
+def check_packed(m, lens, state, out, new, cu0=0):
+    H, P = m["x"].shape[1:]
+    Ns = m["B"].shape[2]
+    at = cu0
+    for i, n in enumerate(lens):
+        S0 = state[i] if state is not None else torch.zeros(H, P, Ns)
+        seq = {k: m[k][at:at + n] for k in ("x", "B", "C", "a")}
+        y, ya, S, Sa = L.scan_ref(**seq, A_log=m["A_log"], dt_bias=m["dt_bias"], D=m["D"], S=S0)
+        L.within(out[at:at + n], y, y_slack(ya, n))
+        L.within(new[i], S, s_slack(Sa, n))
+        at += n
+
+
+@pytest.mark.parametrize("H,P,G,Ns", [(2, 64, 1, 128), (3, 64, 1, 128), (6, 64, 2, 64), (2, 128, 1, 128),
+                                      (4, 128, 2, 64), (1, 64, 1, 64)])
+@pytest.mark.parametrize("lens,state", [([1], False), ([1, 0, 2, 63, 64, 65], True), ([0, 200, 1, 0, 130], True),
+                                        ([127, 128, 129], False), ([700], True)])
+def test_packed(lens, state, H, P, G, Ns):
+    from gdn_b200 import ssm
+    m = make((sum(lens),), H, P, G, Ns, seed=sum(lens) + H, skip=H != 3)
+    st = torch.randn(len(lens), H, P, Ns, device="cuda") if state else None
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0)
+    out, new = ssm.run(m["x"], m["B"], m["C"], st, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)
+    check_packed(m, lens, st, out, new)
+
+
+def test_rows_of_no_sequence_stay():
+    from gdn_b200 import ssm
+    m = make((300,), 4, 64, 1, 128)
+    out = torch.full((300, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    cu = torch.tensor([5, 80, 80, 281], dtype=torch.int32, device="cuda")
+    _, new = ssm.run(m["x"], m["B"], m["C"], None, m["A_log"], m["a"], m["dt_bias"], m["D"], cu, output=out)
+    assert (out[:5] == 7).all() and (out[281:] == 7).all()
+    check_packed(m, [75, 0, 201], None, out, new, cu0=5)
+    assert (new[1] == 0).all()
+
+
+def test_no_tokens_keeps_the_states():
+    from gdn_b200 import ssm
+    m = make((0,), 2, 64, 1, 128)
+    st = torch.randn(2, 2, 64, 128, device="cuda")
+    cu = torch.zeros(3, dtype=torch.int64, device="cuda")
+    out, new = ssm.run(m["x"], m["B"], m["C"], st, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)
+    assert out.shape == (0, 2, 64) and torch.equal(new, st)
+
+
+def test_strong_and_absent_decay():
+    """Decays from none (dt near 0) to complete within a token (dt A of thousands) leave no infinity or NaN."""
+    from gdn_b200 import ssm
+    lens = [150, 90]
+    m = make((240,), 4, 64, 1, 128, seed=5)
+    m["A_log"] = torch.tensor([-20.0, 0.0, 5.0, 12.0], device="cuda")
+    m["dt_bias"] = torch.tensor([30.0, -30.0, 3.0, 1.0], device="cuda")
+    st = torch.randn(2, 4, 64, 128, device="cuda")
+    cu = torch.tensor([0, 150, 240], device="cuda")
+    out, new = ssm.run(m["x"], m["B"], m["C"], st, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)
+    check_packed(m, lens, st, out, new)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,P,G,Ns", [(4, 64, 2, 128), (3, 64, 1, 64), (2, 128, 1, 128), (2, 128, 2, 64)])
+@pytest.mark.parametrize("B,T", [(1, 1), (5, 1), (3, 4), (2, 17)])
+def test_pool(B, T, H, P, G, Ns, dtype):
+    from gdn_b200 import ssm
+    m = make((B, T), H, P, G, Ns, seed=B * 100 + T, skip=T != 4)
+    pool = torch.randn(B + 3, H, P, Ns, device="cuda").to(dtype)
+    slots = torch.randperm(B + 3, device="cuda")[:B].to(torch.int32)
+    was = pool.clone()
+    args = (m["x"], m["B"], m["C"], m["A_log"], m["a"], m["dt_bias"], m["D"], pool, slots)
+    dry = ssm.run_pool(*args, no_state_update=True)
+    assert torch.equal(pool, was)
+    out = ssm.run_pool(*args)
+    assert torch.equal(out, dry)
+    for i, at in enumerate(slots.tolist()):
+        y, ya, S, Sa = L.scan_ref(*(m[k][i] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"], was[at])
+        L.within(out[i], y, f32_slack(ya, T))
+        L.within(pool[at], S, f32_slack(Sa, T))
+        was[at] = pool[at]
+    assert torch.equal(pool, was), "a slot of no sequence changed"
+
+
+def test_pool_slots():
+    from gdn_b200 import ssm
+    m = make((4, 2), 2, 64, 1, 128)
+    pool = torch.randn(6, 2, 64, 128, device="cuda")
+    was = pool.clone()
+    reads = torch.tensor([-1, 6, 2, 3], dtype=torch.int32, device="cuda")
+    writes = torch.tensor([0, 1, -1, 5], dtype=torch.int32, device="cuda")
+    out = ssm.run_pool(m["x"], m["B"], m["C"], m["A_log"], m["a"], m["dt_bias"], m["D"], pool, reads, writes)
+    for i, (r, w) in enumerate(zip([None, None, 2, 3], [0, 1, None, 5])):
+        S0 = was[r] if r is not None else torch.zeros(2, 64, 128)
+        y, ya, S, Sa = L.scan_ref(*(m[k][i] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"], S0)
+        L.within(out[i], y, f32_slack(ya, 2))
+        if w is not None:
+            L.within(pool[w], S, f32_slack(Sa, 2))
+    assert torch.equal(pool[2:5], was[2:5])
+
+
+def test_tokens_after_a_prompt():
+    """A prompt, then tokens over the pool, against the whole sequence."""
+    from gdn_b200 import ssm
+    T = 150
+    m = make((T,), 4, 64, 2, 128, seed=9)
+    n = 141
+    cu = torch.tensor([0, n], device="cuda")
+    head, state = ssm.run(m["x"][:n], m["B"][:n], m["C"][:n], None, m["A_log"], m["a"][:n], m["dt_bias"], m["D"], cu)
+    slot = torch.zeros(1, dtype=torch.int32, device="cuda")
+    outs = [ssm.run_pool(*(m[k][None, t:e] for k in ("x", "B", "C")), m["A_log"], m["a"][None, t:e], m["dt_bias"],
+                         m["D"], state, slot) for t, e in ((n, n + 1), (n + 1, n + 6), (n + 6, T))]
+    y, ya, S, Sa = L.scan_ref(*(m[k] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"],
+                              torch.zeros(4, 64, 128))
+    L.within(torch.cat([head] + [o[0] for o in outs]), y, y_slack(ya, T))
+    L.within(state[0], S, s_slack(Sa, T))
+
+
+def test_refusals():
+    from gdn_b200 import ssm
+    m = make((10,), 4, 64, 2, 128)
+    cu = torch.tensor([0, 10], device="cuda")
+    ok = dict(x=m["x"], B=m["B"], C=m["C"], state=None, A_log=m["A_log"], a=m["a"], dt_bias=m["dt_bias"], D=m["D"],
+              cu_seqlens=cu)
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    for exc, match, kw in [
+            (TypeError, "x must", dict(x=m["x"].half())),
+            (ValueError, "head size", dict(x=z(10, 4, 32))),
+            (ValueError, "state size", dict(B=z(10, 2, 32), C=z(10, 2, 32))),
+            (ValueError, "multiple", dict(B=z(10, 3, 128), C=z(10, 3, 128))),
+            (ValueError, "C must", dict(C=z(10, 1, 128))),
+            (ValueError, "contiguous", dict(x=z(10, 4, 128)[..., :64])),
+            (TypeError, "A_log", dict(A_log=z(4))),
+            (ValueError, "a must", dict(a=z(9, 4))),
+            (TypeError, "state", dict(state=z(1, 4, 64, 128))),
+            (ValueError, "at least one", dict(cu_seqlens=cu[:1])),
+            (ValueError, "CUDA|same device", dict(B=m["B"].cpu()))]:
+        with pytest.raises(exc, match=match):
+            ssm.run(**{**ok, **kw})
+    st = z(1, 4, 64, 128, dt=torch.float32)
+    with pytest.raises(ValueError, match="overlaps"):
+        ssm.run(**{**ok, "state": st}, new_state=st)
