@@ -408,7 +408,8 @@ int gdn_rms_norm(const void *x, int64_t x_row_stride, const void *weight, const 
 /*
  * Device status word.  A kernel that gives up on a bounded wait (an mbarrier
  * that does not complete within 2 s) sets a bit here and returns instead of
- * hanging: bit 0 = chunked prefill, bit 1 = gdn_wait_probe.  Reads the word of
+ * hanging: bit 0 = chunked prefill, bit 1 = gdn_wait_probe,
+ * bit 2 = pooled decode, bit 3 = gdn_ssm.  Reads the word of
  * the current device (synchronising), optionally clearing it.  No reference
  * counterpart: the reference relies on cudaGetLastError only
  * (gdn_decode_small_batch.cu:223-227).

@@ -517,9 +517,13 @@ static int check_ssm(const void* x, const void* B, const void* C, const float* A
   return GDN_OK;
 }
 
+static bool ssm_recurrent(int64_t T, int64_t N) { return T <= 16 * N; }
+
 size_t gdn_ssm_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P, int64_t Ns) {
-  (void)T, (void)N, (void)H, (void)G, (void)P, (void)Ns;
-  return 0;
+  if (T <= 0 || N <= 0 || H <= 0 || G <= 0 || H % G != 0 || (P != 64 && P != 128) || (Ns != 64 && Ns != 128) ||
+      ssm_recurrent(T, N))
+    return 0;
+  return gdn::ssm_chunked_workspace(T, N, H, G, P, Ns, sm_count());
 }
 
 int gdn_ssm(const void* x, const void* B, const void* C, const float* state, const float* A_log,
@@ -535,12 +539,16 @@ int gdn_ssm(const void* x, const void* B, const void* C, const float* state, con
   if (T > 0x7fffffffLL - 64) return fail(GDN_ERR_VALUE, "total_seq_len too large");
   const size_t bytes = static_cast<size_t>(N) * H * P * Ns * 4;
   if (overlap(state, bytes, new_state, bytes)) return fail(GDN_ERR_VALUE, "new_state overlaps state");
-  (void)workspace, (void)workspace_bytes;
+  const size_t need = gdn_ssm_workspace_bytes(T, N, H, G, P, Ns);
+  if (workspace && workspace_bytes < need) return fail(GDN_ERR_VALUE, "workspace needs %zu bytes", need);
+  if (!aligned(workspace, 256)) return fail(GDN_ERR_VALUE, "workspace must be 256-byte aligned");
   gdn::SsmArgs p{};
   p.x = x, p.B = B, p.C = C, p.state = state, p.A_log = A_log, p.a = a, p.dt_bias = dt_bias, p.D = D;
   p.cu_seqlens = cu_seqlens, p.out = output, p.new_state = new_state;
   p.T = T, p.N = N, p.H = H, p.G = G, p.P = P, p.Ns = Ns;
-  return cuda_status(gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream)), "gdn_ssm launch");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (ssm_recurrent(T, N)) return cuda_status(gdn::launch_ssm_recurrent(p, st), "gdn_ssm launch");
+  return cuda_status(gdn::launch_ssm_chunked(p, need ? workspace : nullptr, sm_count(), st), "gdn_ssm launch");
 }
 
 int gdn_ssm_pool(const void* x, const void* B, const void* C, const float* A_log, const void* a,

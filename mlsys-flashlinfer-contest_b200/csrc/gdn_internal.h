@@ -187,6 +187,11 @@ struct SsmArgs {
 };
 // Token by token on CUDA cores, the state in registers: the pool form and short prompts.
 cudaError_t launch_ssm_recurrent(const SsmArgs& a, cudaStream_t s);
+// Packed prompts in chunks of 64 tokens on tcgen05; `ws` (ssm_chunked_workspace bytes, may be
+// nullptr) lets it cut sequences into pieces when few (sequence, head) pairs would leave SMs idle.
+size_t ssm_chunked_workspace(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P, int64_t Ns, int sms);
+cudaError_t launch_ssm_chunked(const SsmArgs& a, void* ws, int sms, cudaStream_t s);
+cudaError_t read_ssm_status(uint32_t* out, bool clear);
 
 // Root-mean-square norm over rows (gdn_norm.cu).
 struct NormArgs {

@@ -1467,6 +1467,9 @@ cudaError_t read_status(uint32_t* out, bool clear) {
   uint32_t pool = 0;  // the pooled tensor-core decode keeps its own word
   if ((e = read_pool_tc_status(&pool, clear)) != cudaSuccess) return e;
   *out |= pool;
+  uint32_t ssm = 0;  // and so does the selective scan
+  if ((e = read_ssm_status(&ssm, clear)) != cudaSuccess) return e;
+  *out |= ssm;
   if (clear) {
     const uint32_t zero = 0;
     e = cudaMemcpyToSymbol(g_gdn_status, &zero, sizeof(uint32_t));

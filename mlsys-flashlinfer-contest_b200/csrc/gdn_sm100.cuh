@@ -18,6 +18,7 @@ enum : uint32_t {
   kStatusPrefillTimeout = 1u << 0,
   kStatusProbeTimeout = 1u << 1,
   kStatusPoolTimeout = 1u << 2,
+  kStatusSsmTimeout = 1u << 3,
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -172,3 +172,62 @@ def test_refusals():
     st = z(1, 4, 64, 128, dt=torch.float32)
     with pytest.raises(ValueError, match="overlaps"):
         ssm.run(**{**ok, "state": st}, new_state=st)
+
+
+@pytest.fixture(autouse=True)
+def no_timeouts():
+    """No kernel of a test gave up on a bounded wait."""
+    import ctypes
+    from gdn_b200 import _native as N
+    yield
+    status = ctypes.c_uint32()
+    assert N.lib().gdn_read_status(ctypes.byref(status), 1) == N.GDN_OK and status.value == 0
+
+
+@pytest.mark.parametrize("what", ["x nan", "x inf", "a nan", "a inf", "B nan", "C inf"])
+def test_values_that_are_not_finite_stay_where_they_belong(what):
+    """Row h, p from token j on (x), head h from token j on (a), everything of the group from token j on (B), token
+    j of the group (C): nothing earlier, no other head, no other sequence."""
+    from gdn_b200 import ssm
+    H, P, G, Ns = 4, 64, 2, 128
+    lens = [100, 137, 50]
+    m = make((287,), H, P, G, Ns, seed=3)
+    cu = torch.tensor([0, 100, 237, 287], device="cuda")
+    run = lambda m: ssm.run(m["x"], m["B"], m["C"], None, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)  # noqa: E731
+    want, want_s = run(m)
+    for j in (100, 100 + 63, 100 + 70, 236):
+        name, value = what.split()
+        bad = {k: (v.clone() if v is not None else None) for k, v in m.items()}
+        bad[name][(j, 1, 5) if name in ("x", "B", "C") else (j, 1)] = float(value)
+        got, got_s = run(bad)
+        y = torch.zeros(287, H, P, dtype=torch.bool, device="cuda")   # what may (and has to) differ
+        s = torch.zeros(3, H, P, Ns, dtype=torch.bool, device="cuda")
+        if name == "x":
+            y[j:237, 1, 5], s[1, 1, 5] = True, True
+        elif name == "a":
+            y[j:237, 1], s[1, 1] = True, True
+        elif name == "B":
+            y[j:237, 2:], s[1, 2:, :, 5] = True, True
+        else:
+            y[j, 2:] = True
+        assert torch.equal(got[~y], want[~y]), f"{what} at {j} reached other outputs"
+        assert torch.equal(got_s[~s], want_s[~s]), f"{what} at {j} reached other states"
+        assert not got_s[s].isfinite().any()
+        if name != "a" or value == "nan":
+            assert not got[y].isfinite().any()
+
+
+def test_same_answer_twice_and_beside_other_sequences():
+    """Bitwise: no order of execution enters the sums, and a sequence's results do not depend on its neighbours."""
+    from gdn_b200 import ssm
+    lens = [300, 65, 0, 190]
+    m = make((sum(lens),), 6, 64, 2, 128, seed=11)
+    st = torch.randn(4, 6, 64, 128, device="cuda")
+    cu = torch.tensor([0, 300, 365, 365, 555], device="cuda")
+    run = lambda t0, t1, st, cu: ssm.run(m["x"][t0:t1], m["B"][t0:t1], m["C"][t0:t1], st, m["A_log"],  # noqa: E731
+                                         m["a"][t0:t1], m["dt_bias"], m["D"], cu)
+    y, s = run(0, 555, st, cu)
+    y2, s2 = run(0, 555, st, cu)
+    assert torch.equal(y, y2) and torch.equal(s, s2)
+    y3, s3 = run(300, 365, st[1:2], torch.tensor([0, 65], device="cuda"))
+    assert torch.equal(y[300:365], y3) and torch.equal(s[1:2], s3)
