@@ -12,14 +12,16 @@
 //   S     <- e^{gamma_63} S + W^T B,   W = e^{gamma_63 - gamma_j} dt_j x_j
 // Roundings: M and the S that C reads are bf16 operands (their errors, like the output's
 // own rounding, are 2^-8 of a term).  The state itself stays fp32 in registers for the whole
-// piece, and W enters its update as two bf16 terms (hi + lo, ~16 bits of mantissa; B is bf16
-// already), so the fp32 final state keeps ~2^-17.
+// piece, and W enters its update as three bf16 terms (24 bits of mantissa; B is bf16
+// already): the final state is as exact as fp32 sums make it.  Two terms left 2.6e-6 of it.
 //
-// The decays between a row and the columns of a 16-column block are r_i u_j with
-// u_j = dt_j e^{gamma_top - gamma_j} (a table, top = the block's last column) and
-// r_i = e^{gamma_i - gamma_top} below the diagonal; in blocks on the diagonal, where that
-// could overflow, they are walked down each four columns from the highest j <= i.  No
-// factor exceeds 1, whatever the decay.
+// The decays between a row and the columns of a 16-column block are r_i u_j.  Below the
+// diagonal u_j = dt_j e^{gamma_top - gamma_j} (a table, top = the block's last column) and
+// r_i = e^{gamma_i - gamma_top}: no factor exceeds 1, whatever the decay.  In the blocks on the
+// diagonal both refer to the block's first column instead, which u_j may exceed by the
+// block's decay; where that is more than 2^64 (a flag of the tables), each element gets its own
+// exponential.  The mask and the skip term D of a row come from tables in shared memory (a mask
+// word per two columns, applied to the packed bf16 values, so that it also hides a NaN).
 //
 // Values that are not finite stay where the recurrence puts them.  A masked factor 0 times
 // an infinite x would leak into earlier tokens, and 0 times a NaN weight into the other
@@ -28,10 +30,15 @@
 // the decays (e^gamma and the chunk's); tokens past the end are zeroed in x and B.
 //
 // Warp roles: warps 0-15 compute (four per TMEM lane quarter, each on a quarter of the
-// columns), warp 16 issues the MMAs and the output's TMA stores, warp 17 the TMA loads.
-// The compute warps run, for chunk c: the operands W (quarters 0-1) and M (quarters 2-3)
-// of chunk c + 1, the outputs of chunk c, the state update of chunk c.  Each step's matrix
-// products were issued a step earlier, so no step waits for one to run.
+// columns), warp 16 issues the MMAs, warp 17 the TMA loads, warps 18-19 compute the gate
+// tables of a head each.  The compute warps run, for chunk c: the operands W (quarters
+// 0-1) and M (quarters 2-3) of chunk c + 1, the outputs of chunk c, the state update of
+// chunk c.  Each step's matrix products were issued a step earlier, so no step waits for one
+// to run, and warps meet through mbarriers only (they may be in different steps).
+// What bounds the kernel is the compute warps' instructions, not HBM or the tensor pipe:
+// W ~60 a 16-byte piece of x (three terms), M ~45 a 32 x 16 block and head.  Outputs go from
+// registers to HBM: a warp's store covers two 64-byte row pieces, so nothing is gained by a tile
+// in shared memory, whose 16 KiB hold the third term of W instead.
 //
 // Few (sequence, head tile) pairs: sequences are cut into pieces of `seg` tokens.  A first
 // launch (STATE_ONLY) finds each piece's final state from zero and its decay; the second runs
@@ -39,6 +46,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <string.h>
+#include <type_traits>
 
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
@@ -53,12 +61,12 @@ using namespace sm100;
 
 constexpr int kComputeWarps = 16;
 constexpr int kComputeThreads = 32 * kComputeWarps;
-constexpr int kMmaWarp = 16;  // then the load warp
-constexpr int kThreads = kComputeThreads + 64;
-constexpr uint32_t kComputeBar = 1;
+constexpr int kMmaWarp = 16, kGateWarp = 18;  // 17: TMA loads, 19: the second head's gates
+constexpr int kThreads = kComputeThreads + 128;
 constexpr uint64_t kTimeoutNs = 2000000000ull;  // 2 s per wait, then give up
 constexpr int kStages = 3;
 constexpr int kRows = 128;  // state rows of a CTA
+constexpr int kTerms = 3;   // bf16 terms of W
 
 // ---- TMEM columns ----------------------------------------------------------
 constexpr uint32_t TM_G = 0;     // lanes 64-127: G [i][j]
@@ -70,13 +78,12 @@ constexpr uint32_t kTmemCols = 512;
 
 // ---- per-token tables (floats) of one head and chunk ------------------------
 constexpr int G_GAM = 0;    // gamma, in log2 units
-constexpr int G_D = 64;     // 2^(gamma_t - gamma_{t-1})
+constexpr int G_V = 64;     // dt 2^(gamma of the first token of t's 16 - gamma_t)
 constexpr int G_DT = 128;   // dt (0 past the end)
 constexpr int G_U = 192;    // dt 2^(gamma of the last token of t's 16 - gamma_t)
 constexpr int G_W = 256;    // dt 2^(gamma_63 - gamma_t)
 constexpr int G_EG = 320;   // 2^gamma_t
 constexpr int kGateFloats = 384;
-constexpr int kGateBufs = 3;
 
 // ---- shared memory (offsets from a 1024-aligned base) ------------------------
 template <int P, int NS>
@@ -88,23 +95,33 @@ struct Lay {
   static constexpr uint32_t OFF_Z0 = 0;      // 2 KiB of zeros below the stages ...
   static constexpr uint32_t OFF_ST = 2048;
   static constexpr uint32_t OFF_Z1 = OFF_ST + kStages * kStage;  // ... and above
-  static constexpr uint32_t OFF_W = OFF_Z1 + 2048;    // W hi, then lo: [block 2][t 64][128 B]
-  static constexpr uint32_t OFF_M = OFF_W + 32768;    // M of each head: [i 64][128 B]
-  static constexpr uint32_t OFF_Y = OFF_M + 16384;    // outputs [block 2][t 64][128 B]
-  static constexpr uint32_t OFF_G = OFF_Y + 16384;    // tables [buffer][head][kGateFloats]
-  static constexpr uint32_t OFF_DEC = OFF_G + kGateBufs * 2 * kGateFloats * 4;  // [buffer][head]
-  static constexpr uint32_t OFF_BAD = OFF_DEC + 32;   // first token whose x is not finite, by row
-  static constexpr uint32_t OFF_BAR = OFF_BAD + kRows * 4;
+  static constexpr uint32_t OFF_W = OFF_Z1 + 2048;    // the terms of W: [term 3][block 2][t 64][128 B]
+  static constexpr uint32_t OFF_M = OFF_W + kTerms * 16384;  // M of each head: [i 64][128 B]
+  static constexpr uint32_t OFF_G = OFF_M + 16384;    // tables [buffer][head][kGateFloats]
+  static constexpr uint32_t OFF_DEC = OFF_G + kStages * 2 * kGateFloats * 4;  // [buffer][head]
+  static constexpr uint32_t OFF_STEEP = OFF_DEC + 32;  // [buffer][head]: a bit per 16-block of G_V out of range
+  static constexpr uint32_t OFF_BAD = OFF_STEEP + 32;  // first token whose x is not finite, by row
+  // by a row's distance from its block's first column, clamped to -1..16 (row 0 is -1): mask
+  // words of the 16 columns, and D at the diagonal of each head (pitches free of bank conflicts)
+  static constexpr uint32_t OFF_MASK = OFF_BAD + kRows * 4;
+  static constexpr uint32_t kMaskPitch = 48, kSkipPitch = 80, kSkipHead = 18 * kSkipPitch;
+  static constexpr uint32_t OFF_SKIP = OFF_MASK + 18 * kMaskPitch;
+  static constexpr uint32_t OFF_BAR = OFF_SKIP + 2 * kSkipHead;
   static constexpr uint32_t kBytes = OFF_BAR + 256 + 1024;
 };
 static_assert(Lay<64, 128>::kBytes <= 232448, "shared memory");
 
 enum : int {
-  B_FULL = 0,               // kStages: TMA loads landed
-  B_EMPTY = B_FULL + kStages,  // kStages: every product that reads the stage is done
-  B_RDY_W = B_EMPTY + kStages, B_RDY_M, B_RDY_D, B_RDY_S,  // compute warps -> issue warp
-  B_G, B_DS, B_DS1, B_PV, B_QS, B_END, kNumBars            // products done
+  B_BC = 0,                 // kStages: a chunk's B and C landed
+  B_X = B_BC + kStages,     // kStages: its x landed and its tables are written
+  B_EMPTY = B_X + kStages,  // kStages: every product that reads the stage is done
+  B_DONE = B_EMPTY + kStages,  // kStages: the compute warps are through with a chunk, and with the
+                               // state that the next one reads
+  B_START = B_DONE + kStages,  // the state that chunk 0 reads
+  B_RDY_W, B_RDY_M, B_RDY_D,   // compute warps -> issue warp
+  B_G, B_DS, B_DS1, B_PV, B_QS, B_END, kNumBars  // products done
 };
+static_assert(kNumBars * 8 + 12 <= 256, "barrier area");
 
 struct Params {
   const float* state;
@@ -132,6 +149,61 @@ __device__ __forceinline__ void load16(const float* src, float* v) {
     v[4 * q + 3] = x.w;
   }
 }
+
+// Shared-memory store of an operand that only the tensor pipe reads: without a compiler barrier,
+// so that loads of tables and the arithmetic of the next piece may pass it.
+__device__ __forceinline__ void sts128_op(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d));
+}
+
+__device__ __forceinline__ void sts32_op(uint32_t addr, uint32_t a) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(a));
+}
+
+// The MMAs are issued from code that the whole warp runs, each instruction by one lane
+// (`leader`): descriptors then stay in uniform registers.  In a branch of one lane every
+// descriptor is built in vector registers and moved over, ~100 cycles an MMA.
+__device__ __forceinline__ void mma_ss_by(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_by(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit_by(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+// One lane of the (converged) warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+
+// The long form of a wait, out of line: polls with short naps, gives up after kTimeoutNs.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait_nap(bar, parity, kTimeoutNs); }
 
 struct Piece {
   int64_t seq, bos, eos;  // sequence (-1: none) and the piece's tokens
@@ -193,12 +265,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Lay<P, NS>;
   constexpr int kHeads = L::kHeads, kKb = L::kKb;
   constexpr int kCols = NS / 4;  // state columns of a compute thread
-  constexpr int kWWarps = STATE_ONLY ? kComputeWarps : 8;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sb = smem_u32(smem);
   float* gates = reinterpret_cast<float*>(smem + L::OFF_G);
   float* decs = reinterpret_cast<float*>(smem + L::OFF_DEC);
+  uint32_t* steep = reinterpret_cast<uint32_t*>(smem + L::OFF_STEEP);
   int* first_bad = reinterpret_cast<int*>(smem + L::OFF_BAD);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
@@ -240,7 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kNumBars; ++i)
-      mbar_init(&bars[i], i == B_RDY_W ? kWWarps : i == B_RDY_M ? 8 : (i == B_RDY_D || i == B_RDY_S) ? kComputeWarps : 1);
+      mbar_init(&bars[i], i == B_RDY_W ? (STATE_ONLY ? kComputeWarps : 12) : i == B_RDY_M ? 6
+                         : (i == B_RDY_D || (i >= B_DONE && i <= B_START)) ? kComputeWarps
+                         : i >= B_X && i < B_EMPTY ? 1 + kHeads : 1);
     fence_mbar_init();
     *abort_flag = 0u;
     *any_bad = 0u;
@@ -263,6 +337,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       sts128(sb + L::OFF_Z1 + 16 * i, 0u, 0u, 0u, 0u);
     }
     for (int i = tid; i < 1024; i += kThreads) sts128(sb + L::OFF_M + 16 * i, 0u, 0u, 0u, 0u);
+    for (int i = tid; i < 18 * 16; i += kThreads) {
+      const int d = i / 16 - 1, j = i % 16;
+      reinterpret_cast<uint16_t*>(smem + L::OFF_MASK + (d + 1) * L::kMaskPitch)[j] = j <= d ? 0xffffu : 0u;
+      for (int head = 0; head < kHeads; ++head)
+        reinterpret_cast<float*>(smem + L::OFF_SKIP + head * L::kSkipHead + (d + 1) * L::kSkipPitch)[j] =
+            j == d && p.D && (head == 0 || two) ? p.D[h0 + head] : 0.f;
+    }
   }
   if (kHeads == 2 && !two)  // the absent head's x
     for (int i = tid; i < kStages * 512; i += kThreads)
@@ -283,88 +364,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[b]);
     };
+    // After a timeout a thread waits for nothing any more (its results are garbage, the status
+    // word says so) and leaves the loop.
     auto wait = [&](int b, uint32_t parity) {
-      if (!failed) failed = !mbar_wait_nap(&bars[b], parity, kTimeoutNs);
+      if (!failed && !mbar_test(&bars[b], parity)) failed = !wait_long(&bars[b], parity);
       tc_fence_after();
     };
-    auto table = [&](int c, int head) { return gates + ((c % kGateBufs) * 2 + head) * kGateFloats; };
-
-    // ---- gates: warp 10 computes head 0's tables, warp 14 head 1's (quarter 2, the columns
-    //      of M above the diagonal, where there is nothing else to do) ---------------
-    const bool gate_warp = quarter == 2 && (cq == 2 || (cq == 3 && kHeads == 2));
-    const int gh = cq - 2;
-    const bool gate_live = gate_warp && (gh == 0 || two);
-    float negA = 0.f, bias = 0.f;
-    unsigned short raw[2] = {0, 0};
-    if (gate_live) {
-      negA = -expf(p.A_log[h0 + gh]) * kLog2e;
-      bias = p.dt_bias[h0 + gh];
-    }
-    auto prefetch_gates = [&](int c) {
-      if (!gate_live) return;
-      const unsigned short* pa = reinterpret_cast<const unsigned short*>(p.a);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t t = bos + static_cast<int64_t>(c) * kChunk + 2 * lane + e;
-        if (t < pc.eos) raw[e] = pa[t * p.H + h0 + gh];
-      }
-    };
-    auto compute_gates = [&](int c) {
-      const int Lc = gate_live ? static_cast<int>(min(static_cast<int64_t>(kChunk), Ltot - static_cast<int64_t>(c) * kChunk)) : 0;
-      float dt[2], lg[2];
-      bool ok[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool valid = 2 * lane + e < Lc;
-        dt[e] = valid ? softplus_t20(bf16_bits_to_f32(raw[e]) + bias) : 0.f;
-        lg[e] = valid ? negA * dt[e] : 0.f;
-        ok[e] = dt[e] < __int_as_float(0x7f800000) && lg[e] == lg[e];
-        // 2^-256 is 0 in fp32: a stronger decay is the same, and sums stay finite
-        lg[e] = ok[e] ? fmaxf(lg[e], -256.f) : 0.f;
-        dt[e] = ok[e] ? dt[e] : 0.f;
-      }
-      const unsigned bad0 = __ballot_sync(0xffffffffu, !ok[0]), bad1 = __ballot_sync(0xffffffffu, !ok[1]);
-      const int fb = min(bad0 ? 2 * (__ffs(bad0) - 1) : 64, bad1 ? 2 * (__ffs(bad1) - 1) + 1 : 64);
-      const float pair = lg[0] + lg[1];
-      float incl = pair, suf = pair;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const float y = __shfl_up_sync(0xffffffffu, incl, d);
-        const float z = __shfl_down_sync(0xffffffffu, suf, d);
-        if (lane >= d) incl += y;
-        if (lane + d < 32) suf += z;
-      }
-      const float gt[2] = {incl - lg[1], incl};
-      // gamma_63 - gamma_t as a sum of its own terms (a difference of two long sums would lose
-      // the weights' precision where the decay is strong)
-      const float after = __shfl_down_sync(0xffffffffu, suf, 1);
-      const float tail1 = lane == 31 ? 0.f : after;
-      const float rest[2] = {tail1 + lg[1], tail1};
-      const float top = __shfl_sync(0xffffffffu, gt[1], lane | 7);
-      const float g63 = __shfl_sync(0xffffffffu, gt[1], 31);
-      float* tb = table(c, gh);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int t = 2 * lane + e;
-        tb[G_GAM + t] = gt[e];
-        tb[G_D + t] = ex2_ftz(lg[e]);
-        tb[G_DT + t] = dt[e];
-        tb[G_U + t] = dt[e] * ex2_ftz(top - gt[e]);
-        tb[G_W + t] = dt[e] * ex2_ftz(rest[e]);
-        tb[G_EG + t] = t >= fb ? __int_as_float(0x7fc00000) : ex2_ftz(gt[e]);
-      }
-      if (lane == 0) decs[(c % kGateBufs) * 2 + gh] = fb < 64 ? __int_as_float(0x7fc00000) : ex2_ftz(g63);
-    };
-
-    if (gate_warp) {
-      prefetch_gates(0);
-      compute_gates(0);
-      if (n > 1) {
-        prefetch_gates(1);
-        compute_gates(1);
-      }
-      if (n > 2) prefetch_gates(2);
-    }
+    auto table = [&](int buf, int head) { return gates + (buf * 2 + head) * kGateFloats; };
 
     // ---- initial state ------------------------------------------------------
     float s[kCols];
@@ -406,131 +412,180 @@ __global__ void __launch_bounds__(kThreads, 1)
       else
         tmem_st8u(tl + TM_SB + 8 * cq, w);
       tmem_wait_st();
-      signal(B_RDY_S, false);
     };
-    if (!STATE_ONLY) publish_state();
+    if (!STATE_ONLY) {
+      publish_state();
+      signal(B_START, false);
+    }
 
-    // ---- W of chunk c ---------------------------------------------------------
-    const int wtid = STATE_ONLY ? tid : (warp >> 2) * 64 + (warp & 1) * 32 + lane;  // among the W warps
-    auto make_w = [&](int c) {
-      const uint32_t xs = sb + L::OFF_ST + (c % kStages) * L::kStage;
-      wait(B_FULL + c % kStages, static_cast<uint32_t>((c / kStages) & 1));
-      if (c > 0) wait(B_DS + ((c - 1) & 1), static_cast<uint32_t>(((c - 1) >> 1) & 1));  // W is free
+    // ---- W of chunk c, in 16-byte pieces of x (a warp takes two tokens at a time, a token on 16
+    //      lanes).  The warps of quarters 0-1 take three such pairs, 16 tokens apart; the four
+    //      whose part of M is above or below the diagonal two, 8 apart; those on the diagonal
+    //      none.  (STATE_ONLY: two each, 32 apart.) -----------------------------------
+    const bool w_all = quarter < 2, w_some = (quarter == 2 && cq >= 2) || (quarter == 3 && cq < 2);
+    const int wt = (STATE_ONLY ? 2 * warp : w_all ? (warp >> 2) * 4 + (warp & 1) * 2 : 48 + 2 * ((quarter & 1) * 2 + (cq & 1))) +
+                   (lane >> 4);
+    const int wblk = (lane >> 3) & 1;
+    const uint32_t woff = wblk * 8192 + sw128_off(wt, lane & 7);
+    auto make_w = [&](auto stride, auto count, int c, int st, uint32_t st_par) {
+      constexpr int kStride = decltype(stride)::value, kCount = decltype(count)::value;
+      const uint32_t xs = sb + L::OFF_ST + st * L::kStage + woff;
       const int Lc = static_cast<int>(min(static_cast<int64_t>(kChunk), Ltot - static_cast<int64_t>(c) * kChunk));
-      constexpr int kUnits = 1024 / (32 * kWWarps);
+      wait(B_X + st, st_par);
+      uint4 x[kCount];
+      float w[kCount];
 #pragma unroll
-      for (int k = 0; k < kUnits; ++k) {
-        const int idx = wtid + 32 * kWWarps * k;
-        const int t = idx >> 4, blk = (idx >> 3) & 1;
-        const uint32_t off = blk * 8192 + sw128_off(t, idx & 7);
-        uint4 x = lds128(xs + off);
-        if (t >= Lc) {  // past the end: x and B of the last chunk become zero
-          x = make_uint4(0, 0, 0, 0);
-          sts128(xs + off, 0u, 0u, 0u, 0u);
-          if (blk < kKb) sts128(xs + L::kX + blk * 16384 + sw128_off(t, idx & 7), 0u, 0u, 0u, 0u);
-        }
-        const float w = table(c, kHeads == 2 ? blk : 0)[G_W + t];
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-        uint32_t hi[4], lo[4];
-        float2 chk = make_float2(0.f, 0.f);
+      for (int k = 0; k < kCount; ++k) {
+        x[k] = lds128(xs + k * (kStride * 128));
+        w[k] = table(st, kHeads == 2 ? wblk : 0)[G_W + wt + kStride * k];
+      }
+      if (Lc < kChunk) {  // tokens past the end: x and B become zero
+        wait(B_BC + st, st_par);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 v = __fmul2_rn(make_float2(bf16_lo(xw[e]), bf16_hi(xw[e])), make_float2(w, w));
-          hi[e] = pack_bf16x2(v.x, v.y);
-          const float2 r = __fadd2_rn(v, make_float2(-bf16_lo(hi[e]), -bf16_hi(hi[e])));
-          lo[e] = pack_bf16x2(r.x, r.y);
-          chk = __ffma2_rn(r, make_float2(0.f, 0.f), chk);  // NaN where x is not finite
-        }
-        sts128(sb + L::OFF_W + off, hi[0], hi[1], hi[2], hi[3]);
-        sts128(sb + L::OFF_W + 16384 + off, lo[0], lo[1], lo[2], lo[3]);
-        if (!STATE_ONLY && !(chk.x + chk.y == 0.f)) {
-          uint32_t cl[4];
+        for (int k = 0; k < kCount; ++k)
+          if (wt + kStride * k >= Lc) {
+            x[k] = make_uint4(0, 0, 0, 0);
+            sts128(xs + k * (kStride * 128), 0u, 0u, 0u, 0u);
+            if (wblk < kKb)  // (block wblk of B lies 16 KiB apart, of x 8 KiB)
+              sts128(xs + L::kX + wblk * 8192 + k * (kStride * 128), 0u, 0u, 0u, 0u);
+          }
+      }
+      if (c > 0) wait(B_DS + ((c - 1) & 1), static_cast<uint32_t>(((c - 1) >> 1) & 1));  // W is free
+      float2 chk = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kCount; ++k) {
+        const uint32_t xw[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+        float2 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = __fmul2_rn(make_float2(bf16_lo(xw[e]), bf16_hi(xw[e])), make_float2(w[k], w[k]));
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {  // the rounded value, then what it left
+          uint32_t b[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            cl[e] = xw[e];
+            b[e] = pack_bf16x2(v[e].x, v[e].y);
+            if (term + 1 < kTerms)  // (a product with -1: packed operands have no sign modifier)
+              v[e] = __ffma2_rn(make_float2(bf16_lo(b[e]), bf16_hi(b[e])), make_float2(-1.f, -1.f), v[e]);
+            else
+              chk = __fadd2_rn(chk, v[e]);  // the last remainders: NaN where x is not finite
+          }
+          sts128_op(sb + L::OFF_W + woff + term * 16384 + k * (kStride * 128), b[0], b[1], b[2], b[3]);
+        }
+      }
+      if (!STATE_ONLY && !(chk.x + chk.y == chk.x + chk.y)) {
+#pragma unroll 1
+        for (int k = 0; k < kCount; ++k) {
+          const uint4 xr = lds128(xs + k * (kStride * 128));
+          uint32_t xw[4] = {xr.x, xr.y, xr.z, xr.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int f = 0; f < 2; ++f)
               if (((xw[e] >> (16 * f)) & 0x7f80u) == 0x7f80u) {
-                cl[e] &= f ? 0x0000ffffu : 0xffff0000u;
-                atomicMin(&first_bad[blk * 64 + 8 * (idx & 7) + 2 * e + f], c * kChunk + t);
+                xw[e] &= f ? 0x0000ffffu : 0xffff0000u;
+                atomicMin(&first_bad[wblk * 64 + 8 * (lane & 7) + 2 * e + f], c * kChunk + wt + kStride * k);
                 *any_bad = 1u;
               }
-          }
-          sts128(xs + off, cl[0], cl[1], cl[2], cl[3]);
+          sts128(xs + k * (kStride * 128), xw[0], xw[1], xw[2], xw[3]);
         }
       }
       signal(B_RDY_W, true);
     };
 
     // ---- M of chunk c (quarters 2-3: rows i = row - 64, columns [16 cq, 16 cq + 16)) ----
-    auto make_m = [&](int c) {
+    const int mi = row - 64, r0 = 16 * cq;
+    const int md = min(max(mi - r0, -1), 16) + 1;  // row of the mask and skip tables
+    auto make_m = [&](auto below, int c, int st, uint32_t st_par) {
+      constexpr bool kBelow = decltype(below)::value;  // the block lies below the diagonal
       const uint32_t par = static_cast<uint32_t>(c & 1);
-      if (quarter == 2 && cq >= 2) {  // above the diagonal: zero since the start
-        signal(B_RDY_M, false);
-        return;
+      if (!kBelow) wait(B_X + st, st_par);  // (the tables)
+      float r[kHeads];
+      uint32_t far = 0;
+#pragma unroll
+      for (int head = 0; head < kHeads; ++head) {
+        const float* tb = table(st, head);
+        r[head] = ex2_ftz(tb[G_GAM + mi] - tb[G_GAM + r0 + (kBelow ? 15 : 0)]);
+        if (!kBelow) far |= (steep[st * 2 + head] >> cq & 1u) << head;
       }
-      const int i = row - 64, r0 = 16 * cq;
+      if (c > 0) wait(B_PV, par ^ 1u);  // M is free
       wait(B_G, par);
       float v[16];
       tmem_ld16(tl + TM_G + r0, v);
       tmem_wait_ld();
       reg_fence(v);
-      if (c > 0) wait(B_PV, par ^ 1u);  // M is free
 #pragma unroll
       for (int head = 0; head < kHeads; ++head) {
-        const float* tb = table(c, head);
-        float m[16];
-        if (quarter == 3 && cq < 2) {  // below the diagonal
-          const float r = ex2_ftz(tb[G_GAM + i] - tb[G_GAM + r0 + 15]);
+        const float* tb = table(st, head);
+        uint32_t m[8];
+        if constexpr (kBelow) {
           float u[16];
           load16(tb + G_U + r0, u);
 #pragma unroll
-          for (int jj = 0; jj < 16; jj += 2) {
-            const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v[jj], v[jj + 1]), make_float2(u[jj], u[jj + 1])),
-                                        make_float2(r, r));
-            m[jj] = q.x;
-            m[jj + 1] = q.y;
+          for (int k = 0; k < 8; ++k) {
+            const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
+                                        make_float2(r[head], r[head]));
+            m[k] = pack_bf16x2(q.x, q.y);
           }
         } else {
-          const float gi = tb[G_GAM + i];
-          const float skip = p.D && (head == 0 || two) ? p.D[h0 + head] : 0.f;
-          float dd[16], dt[16];
-          load16(tb + G_D + r0, dd);
-          load16(tb + G_DT + r0, dt);
+          float skip[16];
+          load16(reinterpret_cast<const float*>(smem + L::OFF_SKIP + head * L::kSkipHead + md * L::kSkipPitch), skip);
+          float2 q[8];
+          if (!(far >> head & 1u)) {
+            float u[16];
+            load16(tb + G_V + r0, u);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int topc = r0 + 4 * q + 3;
-            float e = topc <= i ? ex2_ftz(gi - tb[G_GAM + topc]) : 1.f;
+            for (int k = 0; k < 8; ++k)
+              q[k] = __ffma2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
+                                make_float2(r[head], r[head]), make_float2(skip[2 * k], skip[2 * k + 1]));
+          } else {
+            const float gi = tb[G_GAM + mi];
 #pragma unroll
-            for (int jj = 4 * q + 3; jj >= 4 * q; --jj) {
-              const int j = r0 + jj;
-              m[jj] = j <= i ? fmaf(v[jj], e * dt[jj], j == i ? skip : 0.f) : 0.f;
-              e = j > i ? 1.f : e * dd[jj];
+            for (int k = 0; k < 8; ++k) {
+              const int j = r0 + 2 * k;
+              q[k].x = fmaf(v[2 * k], ex2_ftz(fminf(gi - tb[G_GAM + j], 0.f)) * tb[G_DT + j], skip[2 * k]);
+              q[k].y = fmaf(v[2 * k + 1], ex2_ftz(fminf(gi - tb[G_GAM + j + 1], 0.f)) * tb[G_DT + j + 1], skip[2 * k + 1]);
             }
+          }
+          const uint4* mask = reinterpret_cast<const uint4*>(smem + L::OFF_MASK + md * L::kMaskPitch);
+#pragma unroll
+          for (int k4 = 0; k4 < 2; ++k4) {
+            const uint4 a = mask[k4];
+            m[4 * k4] = pack_bf16x2(q[4 * k4].x, q[4 * k4].y) & a.x;
+            m[4 * k4 + 1] = pack_bf16x2(q[4 * k4 + 1].x, q[4 * k4 + 1].y) & a.y;
+            m[4 * k4 + 2] = pack_bf16x2(q[4 * k4 + 2].x, q[4 * k4 + 2].y) & a.z;
+            m[4 * k4 + 3] = pack_bf16x2(q[4 * k4 + 3].x, q[4 * k4 + 3].y) & a.w;
           }
         }
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2)
-          sts128(sb + L::OFF_M + head * 8192 + sw128_off(i, 2 * cq + c2), pack_bf16x2(m[8 * c2], m[8 * c2 + 1]),
-                 pack_bf16x2(m[8 * c2 + 2], m[8 * c2 + 3]), pack_bf16x2(m[8 * c2 + 4], m[8 * c2 + 5]),
-                 pack_bf16x2(m[8 * c2 + 6], m[8 * c2 + 7]));
+          sts128_op(sb + L::OFF_M + head * 8192 + sw128_off(mi, 2 * cq + c2), m[4 * c2], m[4 * c2 + 1], m[4 * c2 + 2],
+                    m[4 * c2 + 3]);
       }
       signal(B_RDY_M, true);
     };
 
-    // ---- outputs of chunk c (row, tokens [16 cq, 16 cq + 16)) -------------------
-    auto outputs = [&](int c) {
+    // ---- outputs of chunk c (row, tokens [16 cq, 16 cq + 16)).  Lanes pair up (row even,
+    //      row + 1) to form bf16x2 words of two rows: at step k the even lane gets token k's, the
+    //      odd lane token 8 + (k ^ 4)'s (the other half of a 128-byte line in the swizzle: no
+    //      bank is met twice).  They go where the chunk's x was, and from there by TMA ----
+    const bool odd = row & 1;
+    const uint32_t pick = odd ? 0x3276u : 0x5410u;
+    const uint32_t ysm = (row >> 6) * 8192 + (16 * cq + (odd ? 8 : 0)) * 128 + 4 * ((row & 7) >> 1);
+    const uint32_t ych = (row & 63) >> 3;
+    auto outputs = [&](int c, int st) {
       const uint32_t par = static_cast<uint32_t>(c & 1);
-      const int Lc = static_cast<int>(min(static_cast<int64_t>(kChunk), Ltot - static_cast<int64_t>(c) * kChunk));
       float eg[16], qs[16], pv[16];
-      load16(table(c, hh) + G_EG + 16 * cq, eg);
-      wait(B_PV, par);
-      tmem_ld16(tl + TM_PV + 16 * cq, pv);
+      load16(table(st, hh) + G_EG + 16 * cq, eg);
+      if (quarter < 2 || (quarter == 2 && cq >= 2) || c + 1 == n) wait(B_PV, par);  // (the others waited for it to write M)
       wait(B_QS, par);
+      const bool bad = *any_bad != 0u;  // (written before this chunk's W was signalled)
+      tmem_ld16(tl + TM_PV + 16 * cq, pv);
       tmem_ld16(tl + TM_QS + 16 * cq, qs);
       tmem_wait_ld();
       reg_fence(pv);
       reg_fence(qs);
+      signal(B_RDY_D, false);
       float o[16];
 #pragma unroll
       for (int k = 0; k < 16; k += 2) {
@@ -539,39 +594,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         o[k] = r.x;
         o[k + 1] = r.y;
       }
-      if (*any_bad) {
+      if (bad) {
         const int fb = first_bad[row] - c * kChunk - 16 * cq;
 #pragma unroll
         for (int k = 0; k < 16; ++k)
           if (k >= fb) o[k] = __int_as_float(0x7fc00000);
       }
-      if (Lc == kChunk) {
-        // lanes pair up (row even, row + 1): the even lane stores the bf16x2 words of the first
-        // eight tokens, the odd lane those of the rest
-        const bool odd = row & 1;
-        const uint32_t ocol = sb + L::OFF_Y + (row >> 6) * 8192 + 4 * ((row & 7) >> 1);
-        const int och = (row & 63) >> 3;
+      uint32_t w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t mine = pack_bf16x2(o[k], o[8 + (k ^ 4)]);
+        w[k] = __byte_perm(mine, __shfl_xor_sync(0xffffffffu, mine, 1), pick);
+      }
+      const int64_t left = Ltot - static_cast<int64_t>(c) * kChunk;
+      if (!row_live) return;
+      if (left >= kChunk) {
+        const uint32_t ys = sb + L::OFF_ST + st * L::kStage + ysm;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {  // token k or k ^ 4 of eight: its row, and its swizzle
+          const uint32_t t = odd ? k ^ 4 : k;
+          sts32_op(ys + t * 128 + ((ych ^ t) << 4), w[k]);
+        }
+      } else {
+        __nv_bfloat16* dst = p.out + ((bos + static_cast<int64_t>(c) * kChunk + 16 * cq + (odd ? 8 : 0)) * p.H + h0 + hh) * P +
+                             (row & (P - 2));
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float mine = odd ? o[8 + k] : o[k];
-          const float theirs = __shfl_xor_sync(0xffffffffu, odd ? o[k] : o[8 + k], 1);
-          const int t = 16 * cq + (odd ? 8 : 0) + k;
-          sts32(ocol + t * 128 + ((och ^ (t & 7)) << 4), odd ? pack_bf16x2(theirs, mine) : pack_bf16x2(mine, theirs));
+          const int t = odd ? k ^ 4 : k;
+          if (16 * cq + (odd ? 8 : 0) + t < left)
+            *reinterpret_cast<uint32_t*>(dst + static_cast<int64_t>(t) * p.H * P) = w[k];
         }
-      } else if (row_live) {
-        __nv_bfloat16* dst = p.out + ((bos + static_cast<int64_t>(c) * kChunk + 16 * cq) * p.H + h0 + hh) * P + (row & (P - 1));
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (16 * cq + k < Lc) dst[static_cast<int64_t>(k) * p.H * P] = __float2bfloat16_rn(o[k]);
       }
-      signal(B_RDY_D, true);
     };
 
     // ---- state update of chunk c ------------------------------------------------
-    auto update = [&](int c) {
-      const float dec = decs[(c % kGateBufs) * 2 + hh];
+    auto update = [&](int c, int st) {
+      const float dec = decs[st * 2 + hh];
       dprod *= dec;
-      wait(B_DS + (c & 1), static_cast<uint32_t>((c >> 1) & 1));
+      if (c + 1 == n || (!STATE_ONLY && !w_all && !w_some))  // (the others waited for it to write W)
+        wait(B_DS + (c & 1), static_cast<uint32_t>((c >> 1) & 1));
       float v[kCols];
       if constexpr (kCols == 32)
         tmem_ld32(tl + TM_DS + 128 * (c & 1) + 32 * cq, v);
@@ -588,31 +649,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!STATE_ONLY && c + 1 < n) publish_state();
     };
 
-    bool aborted = false;
+    // (buffer and stage of chunk c + 1, and their parity)
+    int st = 0, prev = 0;
+    uint32_t st_par = 0;
     for (int c = -1; c < n; ++c) {
-      tc_fence_before();
       if (failed) *abort_flag = 1u;
-      named_sync(kComputeBar, kComputeThreads);  // tables of chunk c + 1; everyone is past chunk c - 1
-      tc_fence_after();
       if (*abort_flag) {
-        aborted = true;
+        failed = true;
         break;
       }
       if (c + 1 < n) {
-        if (STATE_ONLY || quarter < 2) make_w(c + 1);
-        if (!STATE_ONLY && quarter >= 2) make_m(c + 1);
-      }
-      if (gate_warp && c >= 0 && c + 2 < n) {
-        compute_gates(c + 2);
-        if (c + 3 < n) prefetch_gates(c + 3);
+        using std::integral_constant;
+        if (STATE_ONLY) {
+          make_w(integral_constant<int, 32>{}, integral_constant<int, 2>{}, c + 1, st, st_par);
+        } else if (w_all) {
+          make_w(integral_constant<int, 16>{}, integral_constant<int, 3>{}, c + 1, st, st_par);
+        } else {
+          if (w_some) make_w(integral_constant<int, 8>{}, integral_constant<int, 2>{}, c + 1, st, st_par);
+          if (quarter == 3 && cq < 2)
+            make_m(std::true_type{}, c + 1, st, st_par);
+          else if (!w_some)
+            make_m(std::false_type{}, c + 1, st, st_par);
+        }
       }
       if (c >= 0) {
-        if (!STATE_ONLY) outputs(c);
-        update(c);
+        if (!STATE_ONLY) outputs(c, prev);
+        update(c, prev);
+        signal(B_DONE + prev, !STATE_ONLY);
+      }
+      prev = st;
+      if (++st == kStages) {
+        st = 0;
+        st_par ^= 1u;
       }
     }
 
-    if (!aborted && !failed) {
+    if (!failed) {
       if (STATE_ONLY) {
         const int64_t u = slot * p.tiles + tile;
         float4* F = reinterpret_cast<float4*>(p.ws) + u * (kRows * NS / 4) + tid;
@@ -627,136 +699,251 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      // ======================= MMA issue thread ================================
-      constexpr uint32_t idesc_g = idesc_bf16(128, 64, false, false);   // [B; C] B^T
-      constexpr uint32_t idesc_ds = idesc_bf16(128, NS, true, true);    // W^T B
-      constexpr uint32_t idesc_qs = idesc_bf16(128, 64, false, false);  // S (TMEM) C^T
-      constexpr uint32_t idesc_pv = idesc_bf16(128, 64, true, false);   // X^T M^T
-      const uint32_t sb16 = sb >> 4;
-      auto bc16 = [&](int c) { return sb16 + (L::OFF_ST + (c % kStages) * L::kStage + L::kX) / 16; };
-      auto wait = [&](int b, uint32_t parity) -> bool {
-        if (!mbar_wait(&bars[b], parity, kTimeoutNs)) return false;
-        tc_fence_after();
-        return true;
-      };
-      auto mma_g = [&](int c) -> bool {
-        if (!wait(B_FULL + c % kStages, static_cast<uint32_t>((c / kStages) & 1))) return false;
+    // ======================= MMA issue warp ==================================
+    constexpr uint32_t idesc_g = idesc_bf16(128, 64, false, false);   // [B; C] B^T
+    constexpr uint32_t idesc_ds = idesc_bf16(128, NS, true, true);    // W^T B
+    constexpr uint32_t idesc_qs = idesc_bf16(128, 64, false, false);  // S (TMEM) C^T
+    constexpr uint32_t idesc_pv = idesc_bf16(128, 64, true, false);   // X^T M^T
+    const uint32_t leader = elect_one();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);  // (uniform)
+    const uint32_t sb16 = sb >> 4;
+    constexpr uint32_t kStage16 = L::kStage / 16, kBc16 = (L::OFF_ST + L::kX) / 16;
+    auto wait = [&](int b, uint32_t parity) -> bool {
+      const bool done = mbar_test(&bars[b], parity) || wait_long(&bars[b], parity);
+      tc_fence_after();
+      return __all_sync(0xffffffffu, done);
+    };
+    // (st: the chunk's stage)
+    auto mma_g = [&](int st, uint32_t par) -> bool {
+      if (!wait(B_BC + st, par)) return false;
+      const uint32_t bc = sb16 + kBc16 + st * kStage16;
 #pragma unroll
-        for (int ks = 0; ks < NS / 16; ++ks) {
-          const uint64_t d = sdesc_sw128_f(bc16(c) + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16, 16, 1024);
-          mma_bf16_ss(tmem + TM_G, d, d, idesc_g, ks > 0);
-        }
-        mma_commit(&bars[B_G]);
-        return true;
-      };
-      auto mma_ds = [&](int c) {
-        const uint32_t d = tmem + TM_DS + 128 * (c & 1);
+      for (int ks = 0; ks < NS / 16; ++ks) {
+        const uint64_t d = sdesc_sw128_f(bc + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16, 16, 1024);
+        mma_ss_by(leader, tm + TM_G, d, d, idesc_g, ks > 0);
+      }
+      commit_by(leader, &bars[B_G]);
+      return true;
+    };
+    auto mma_ds = [&](int c, int st) {
+      const uint32_t d = tm + TM_DS + 128 * (c & 1), bc = sb16 + kBc16 + st * kStage16;
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+      for (int part = 0; part < kTerms; ++part)
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            mma_bf16_ss(d, sdesc_sw128_f(sb16 + (L::OFF_W + part * 16384 + ks * 2048) / 16, 8192, 1024),
-                        sdesc_sw128_f(bc16(c) + ks * 128, 16384, 1024), idesc_ds, part > 0 || ks > 0);
-        mma_commit(&bars[B_DS + (c & 1)]);
-      };
-      auto mma_pv = [&](int c) {
-        const uint32_t xo = L::OFF_ST + (c % kStages) * L::kStage;
+        for (int ks = 0; ks < 4; ++ks)
+          mma_ss_by(leader, d, sdesc_sw128_f(sb16 + (L::OFF_W + part * 16384 + ks * 2048) / 16, 8192, 1024),
+                    sdesc_sw128_f(bc + ks * 128, 16384, 1024), idesc_ds, part > 0 || ks > 0);
+      commit_by(leader, &bars[B_DS + (c & 1)]);
+    };
+    auto mma_pv = [&](int st) {
+      const uint32_t xo = L::OFF_ST + st * L::kStage;
 #pragma unroll
-        for (int head = 0; head < kHeads; ++head)
+      for (int head = 0; head < kHeads; ++head)
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint64_t b = sdesc_sw128_f(sb16 + (L::OFF_M + head * 8192 + ks * 32) / 16, 16, 1024);
-            // rows 0-63 and 64-127 of X^T are two blocks of 64; with two heads, the block of the
-            // other head is 2 KiB of zeros, so that each head's M meets its own x only
-            uint32_t start = xo + ks * 2048, lbo = 8192;
-            if (kHeads == 2 && head == 0) lbo = L::OFF_Z1 - start;
-            if (kHeads == 2 && head == 1) {
-              lbo = start + 8192 - L::OFF_Z0;
-              start = L::OFF_Z0;
-            }
-            mma_bf16_ss(tmem + TM_PV, sdesc_sw128_f(sb16 + start / 16, lbo, 1024), b, idesc_pv, head > 0 || ks > 0);
+        for (int ks = 0; ks < 4; ++ks) {
+          const uint64_t b = sdesc_sw128_f(sb16 + (L::OFF_M + head * 8192 + ks * 32) / 16, 16, 1024);
+          // rows 0-63 and 64-127 of X^T are two blocks of 64; with two heads, the block of the
+          // other head is 2 KiB of zeros, so that each head's M meets its own x only
+          uint32_t start = xo + ks * 2048, lbo = 8192;
+          if (kHeads == 2 && head == 0) lbo = L::OFF_Z1 - start;
+          if (kHeads == 2 && head == 1) {
+            lbo = start + 8192 - L::OFF_Z0;
+            start = L::OFF_Z0;
           }
-      };
-      auto mma_qs = [&](int c) {
-#pragma unroll
-        for (int ks = 0; ks < NS / 16; ++ks)
-          mma_bf16_ts(tmem + TM_QS, tmem + TM_SB + 8 * ks,
-                      sdesc_sw128_f(bc16(c) + ((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) / 16, 16, 1024), idesc_qs, ks > 0);
-      };
-      bool ok = STATE_ONLY || mma_g(0);
-      for (int c = -1; ok && c < n; ++c) {
-        const uint32_t next = static_cast<uint32_t>((c + 1) & 1);
-        if (c + 1 < n) {
-          if (!(ok = wait(B_RDY_W, next))) break;
-          mma_ds(c + 1);
-          if (STATE_ONLY) {
-            mma_commit(&bars[B_EMPTY + (c + 1) % kStages]);
-          } else {
-            if (!(ok = wait(B_RDY_M, next))) break;
-            if (c + 2 < n && !(ok = mma_g(c + 2))) break;
-          }
+          mma_ss_by(leader, tm + TM_PV, sdesc_sw128_f(sb16 + start / 16, lbo, 1024), b, idesc_pv, head > 0 || ks > 0);
         }
-        if (STATE_ONLY) continue;
+      commit_by(leader, &bars[B_PV]);
+    };
+    auto mma_qs = [&](int st) {
+      const uint32_t bc = sb16 + kBc16 + st * kStage16;
+#pragma unroll
+      for (int ks = 0; ks < NS / 16; ++ks)
+        mma_ts_by(leader, tm + TM_QS, tm + TM_SB + 8 * ks,
+                  sdesc_sw128_f(bc + ((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) / 16, 16, 1024), idesc_qs, ks > 0);
+      commit_by(leader, &bars[B_QS]);
+    };
+    bool ok = STATE_ONLY || mma_g(0, 0);
+    // stages of chunks c, c + 1 and c + 2, and the parities of c's and of c + 2's
+    int s0 = kStages - 1, s1 = 0, s2 = 1;
+    uint32_t par0 = 1, par2 = 0;
+    for (int c = -1; ok && c < n; ++c) {
+      const uint32_t next = static_cast<uint32_t>((c + 1) & 1);
+      if (c + 1 < n) {
+        // (its buffer's readers, the update of chunk c - 1, are done: B_DONE below; with
+        // STATE_ONLY here)
+        if (STATE_ONLY && c >= 1 && !(ok = wait(B_DONE + (c - 1) % kStages, static_cast<uint32_t>(((c - 1) / kStages) & 1))))
+          break;
+        if (STATE_ONLY && !(ok = wait(B_BC + s1, s1 == 0 ? par0 ^ 1u : par0))) break;
+        if (!(ok = wait(B_RDY_W, next))) break;
+        mma_ds(c + 1, s1);
+        if (STATE_ONLY) {
+          commit_by(leader, &bars[B_EMPTY + s1]);
+        } else {
+          if (!(ok = wait(B_RDY_M, next))) break;
+          if (c + 2 < n && !(ok = mma_g(s2, par2))) break;
+        }
+      }
+      if (!STATE_ONLY) {
         if (c >= 0 && !(ok = wait(B_RDY_D, next ^ 1u))) break;  // the outputs of chunk c left their accumulators
         if (c + 1 < n) {
-          mma_pv(c + 1);
-          mma_commit(&bars[B_PV]);
-        }
-        if (c >= 0 && Ltot - static_cast<int64_t>(c) * kChunk >= kChunk) {
-          const int tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
-          tma_store_3d(&tm_y, smem + L::OFF_Y, 0, h0, tok);
-          if (P == 128)
-            tma_store_3d(&tm_y, smem + L::OFF_Y + 8192, 64, h0, tok);
-          else if (two)
-            tma_store_3d(&tm_y, smem + L::OFF_Y + 8192, 0, h0 + 1, tok);
-          bulk_commit();
-        }
-        if (c + 1 < n) {
-          if (!(ok = wait(B_RDY_S, next))) break;
-          mma_qs(c + 1);
-          bulk_wait_read_all();  // the output tile may be written again once B_QS completes
-          mma_commit(&bars[B_QS]);
-          mma_commit(&bars[B_EMPTY + (c + 1) % kStages]);
+          mma_pv(s1);
+          if (!(ok = c < 0 ? wait(B_START, 0) : wait(B_DONE + s0, par0))) break;
+          mma_qs(s1);
+          commit_by(leader, &bars[B_EMPTY + s1]);
         }
       }
-      bulk_wait_all();
-      mma_commit(&bars[B_END]);
-      if (!mbar_wait(&bars[B_END], 0, kTimeoutNs)) ok = false;
-      failed = !ok;
+      s0 = s1;
+      s1 = s2;
+      if (s0 == 0) par0 ^= 1u;
+      if (++s2 == kStages) {
+        s2 = 0;
+        par2 ^= 1u;
+      }
+    }
+    commit_by(leader, &bars[B_END]);
+    failed = !wait(B_END, 0) || !ok;
+  } else if (warp >= kGateWarp) {
+    // ======================= gate tables: warp 18 head 0, warp 19 head 1 =========
+    const int gh = warp - kGateWarp;
+    if (gh < kHeads) {
+      const bool live = gh == 0 || two;
+      const float negA = live ? -expf(p.A_log[h0 + gh]) * kLog2e : 0.f;
+      const float bias = live ? p.dt_bias[h0 + gh] : 0.f;
+      const unsigned short* pa = reinterpret_cast<const unsigned short*>(p.a) + h0 + gh;
+      unsigned short raw[2] = {0, 0};  // two tokens a lane
+      auto load = [&](int c) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t t = bos + static_cast<int64_t>(c) * kChunk + 2 * lane + e;
+          if (live && t < pc.eos) raw[e] = pa[t * p.H];
+        }
+      };
+      load(0);
+      int buf = 0;
+      uint32_t par = 0;
+      for (int c = 0; c < n; ++c) {
+        const int Lc = live ? static_cast<int>(min(static_cast<int64_t>(kChunk), Ltot - static_cast<int64_t>(c) * kChunk)) : 0;
+        float dt[2], lg[2];
+        bool ok[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool valid = 2 * lane + e < Lc;
+          dt[e] = valid ? softplus_t20(bf16_bits_to_f32(raw[e]) + bias) : 0.f;
+          lg[e] = valid ? negA * dt[e] : 0.f;
+          ok[e] = dt[e] < __int_as_float(0x7f800000) && lg[e] == lg[e];
+          // 2^-256 is 0 in fp32: a stronger decay is the same, and sums stay finite
+          lg[e] = ok[e] ? fmaxf(lg[e], -256.f) : 0.f;
+          dt[e] = ok[e] ? dt[e] : 0.f;
+        }
+        if (c + 1 < n) load(c + 1);
+        const unsigned bad0 = __ballot_sync(0xffffffffu, !ok[0]), bad1 = __ballot_sync(0xffffffffu, !ok[1]);
+        const int fb = min(bad0 ? 2 * (__ffs(bad0) - 1) : 64, bad1 ? 2 * (__ffs(bad1) - 1) + 1 : 64);
+        const float pair = lg[0] + lg[1];
+        float incl = pair, suf = pair;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const float y = __shfl_up_sync(0xffffffffu, incl, d);
+          const float z = __shfl_down_sync(0xffffffffu, suf, d);
+          if (lane >= d) incl += y;
+          if (lane + d < 32) suf += z;
+        }
+        const float gt[2] = {incl - lg[1], incl};
+        // gamma_63 - gamma_t as a sum of its own terms (a difference of two long sums would lose
+        // the weights' precision where the decay is strong)
+        const float after = __shfl_down_sync(0xffffffffu, suf, 1);
+        const float tail = lane == 31 ? 0.f : after;
+        const float rest[2] = {tail + lg[1], tail};
+        const float first = __shfl_sync(0xffffffffu, gt[0], lane & 24);
+        const float top = __shfl_sync(0xffffffffu, gt[1], lane | 7);
+        const float g63 = __shfl_sync(0xffffffffu, gt[1], 31);
+        const unsigned far = __ballot_sync(0xffffffffu, first - top > 64.f);
+        if (c >= kStages && !failed && !mbar_test(&bars[B_DONE + buf], par ^ 1u))
+          failed = !wait_long(&bars[B_DONE + buf], par ^ 1u);
+        if (failed) break;
+        float* tb = gates + (buf * 2 + gh) * kGateFloats;
+        *reinterpret_cast<float2*>(tb + G_GAM + 2 * lane) = make_float2(gt[0], gt[1]);
+        *reinterpret_cast<float2*>(tb + G_DT + 2 * lane) = make_float2(dt[0], dt[1]);
+        *reinterpret_cast<float2*>(tb + G_U + 2 * lane) = make_float2(dt[0] * ex2_ftz(top - gt[0]), dt[1] * ex2_ftz(top - gt[1]));
+        *reinterpret_cast<float2*>(tb + G_V + 2 * lane) =
+            make_float2(dt[0] * ex2_ftz(first - gt[0]), dt[1] * ex2_ftz(first - gt[1]));
+        *reinterpret_cast<float2*>(tb + G_W + 2 * lane) = make_float2(dt[0] * ex2_ftz(rest[0]), dt[1] * ex2_ftz(rest[1]));
+        const float nan = __int_as_float(0x7fc00000);
+        *reinterpret_cast<float2*>(tb + G_EG + 2 * lane) =
+            make_float2(2 * lane >= fb ? nan : ex2_ftz(gt[0]), 2 * lane + 1 >= fb ? nan : ex2_ftz(gt[1]));
+        if (lane == 0) {
+          decs[buf * 2 + gh] = fb < 64 ? nan : ex2_ftz(g63);
+          steep[buf * 2 + gh] = (far & 1u) | (far >> 7 & 2u) | (far >> 14 & 4u) | (far >> 21 & 8u);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[B_X + buf]);
+        if (++buf == kStages) {
+          buf = 0;
+          par ^= 1u;
+        }
+      }
     }
   } else if (lane == 0) {
-    // ======================= TMA load thread ===================================
-    const uint32_t bytes = (kHeads == 2 && !two ? 8192u : 16384u) + kKb * (STATE_ONLY ? 8192u : 16384u);
+    // ======================= TMA load and store thread =========================
+    const uint32_t x_bytes = kHeads == 2 && !two ? 8192u : 16384u;
     bool ok = true;
-    int issued = 0;
-    for (int c = 0; ok && c < n; ++c) {
-      const int st = c % kStages;
-      if (c >= kStages && !mbar_wait(&bars[B_EMPTY + st], static_cast<uint32_t>((c / kStages - 1) & 1), kTimeoutNs)) {
-        ok = false;
-        break;
-      }
-      const int tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
-      uint64_t* bar = &bars[B_FULL + st];
-      uint8_t* xs = smem + L::OFF_ST + st * L::kStage;
-      mbar_arrive_expect_tx(bar, bytes);
-      if (P == 128) {
-        tma_load_3d(xs, &tm_x, bar, 0, h0, tok);
-        tma_load_3d(xs + 8192, &tm_x, bar, 64, h0, tok);
-      } else {
-        tma_load_3d(xs, &tm_x, bar, 0, h0, tok);
-        if (two) tma_load_3d(xs + 8192, &tm_x, bar, 0, h0 + 1, tok);
-      }
+    int bc_issued = 0, x_issued = 0;
+    auto load_bc = [&](int c) {
+      const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
+      uint8_t* bc = smem + L::OFF_ST + st * L::kStage + L::kX;
+      mbar_arrive_expect_tx(&bars[B_BC + st], kKb * (STATE_ONLY ? 8192u : 16384u));
 #pragma unroll
       for (int kb = 0; kb < kKb; ++kb) {
-        tma_load_3d(xs + L::kX + kb * 16384, &tm_b, bar, 64 * kb, g, tok);
-        if (!STATE_ONLY) tma_load_3d(xs + L::kX + kb * 16384 + 8192, &tm_c, bar, 64 * kb, g, tok);
+        tma_load_3d(bc + kb * 16384, &tm_b, &bars[B_BC + st], 64 * kb, g, tok);
+        if (!STATE_ONLY) tma_load_3d(bc + kb * 16384 + 8192, &tm_c, &bars[B_BC + st], 64 * kb, g, tok);
       }
-      issued = c + 1;
+      bc_issued = c + 1;
+    };
+    auto load_x = [&](int c) {
+      const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
+      uint8_t* xs = smem + L::OFF_ST + st * L::kStage;
+      mbar_arrive_expect_tx(&bars[B_X + st], x_bytes);
+      tma_load_3d(xs, &tm_x, &bars[B_X + st], 0, h0, tok);
+      if (P == 128)
+        tma_load_3d(xs + 8192, &tm_x, &bars[B_X + st], 64, h0, tok);
+      else if (two)
+        tma_load_3d(xs + 8192, &tm_x, &bars[B_X + st], 0, h0 + 1, tok);
+      x_issued = c + 1;
+    };
+    for (int c = 0; c < min(n, kStages); ++c) {
+      load_bc(c);
+      load_x(c);
     }
-    // no load may be in flight when the CTA ends
-    for (int c = max(0, issued - kStages); c < issued; ++c)
-      if (!mbar_wait(&bars[B_FULL + c % kStages], static_cast<uint32_t>((c / kStages) & 1), kTimeoutNs)) ok = false;
+    for (int c = 0; ok && c < n; ++c) {
+      const int st = c % kStages;
+      const uint32_t par = static_cast<uint32_t>((c / kStages) & 1);
+      if (c + kStages < n) {
+        if (!(ok = mbar_wait(&bars[B_EMPTY + st], par, kTimeoutNs))) break;
+        load_bc(c + kStages);
+        if (STATE_ONLY) load_x(c + kStages);
+      }
+      if (STATE_ONLY) continue;
+      if (!(ok = mbar_wait(&bars[B_DONE + st], par, kTimeoutNs))) break;
+      if (Ltot - static_cast<int64_t>(c) * kChunk >= kChunk) {  // the outputs, where x was
+        const int tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
+        const uint8_t* ys = smem + L::OFF_ST + st * L::kStage;
+        tma_store_3d(&tm_y, ys, 0, h0, tok);
+        if (P == 128)
+          tma_store_3d(&tm_y, ys + 8192, 64, h0, tok);
+        else if (two)
+          tma_store_3d(&tm_y, ys + 8192, 0, h0 + 1, tok);
+        bulk_commit();
+      }
+      if (c + kStages < n) {
+        bulk_wait_read_all();
+        load_x(c + kStages);
+      }
+    }
+    // no copy may be in flight when the CTA ends
+    bulk_wait_all();
+    for (int c = max(0, bc_issued - kStages); c < bc_issued; ++c)
+      if (!mbar_wait(&bars[B_BC + c % kStages], static_cast<uint32_t>((c / kStages) & 1), kTimeoutNs)) ok = false;
+    for (int c = max(0, x_issued - kStages); c < x_issued; ++c)
+      if (!mbar_wait(&bars[B_X + c % kStages], static_cast<uint32_t>((c / kStages) & 1), kTimeoutNs)) ok = false;
     failed = !ok;
   }
   if (failed) atomicOr(&g_ssm_status, kStatusSsmTimeout);
