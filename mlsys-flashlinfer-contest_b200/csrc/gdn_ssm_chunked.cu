@@ -32,7 +32,7 @@
 // Warp roles: warps 0-15 compute (four per TMEM lane quarter, each on a quarter of the
 // columns), warp 16 issues the MMAs, warp 17 the TMA loads, warps 18-19 compute the gate
 // tables of a head each.  The compute warps run, for chunk c: the operands W (quarters
-// 0-1) and M (quarters 2-3) of chunk c + 1, the outputs of chunk c, the state update of
+// 0-1, and pieces elsewhere) and M (quarters 2-3) of chunk c + 1, the state update of chunk c, the outputs of
 // chunk c.  Each step's matrix products were issued a step earlier, so no step waits for one
 // to run, and warps meet through mbarriers only (they may be in different steps).
 // What bounds the kernel is the compute warps' instructions, not HBM or the tensor pipe:
@@ -46,6 +46,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <string.h>
+
+#include <algorithm>
 #include <type_traits>
 
 #include "gdn_common.cuh"
@@ -70,10 +72,10 @@ constexpr int kTerms = 3;   // bf16 terms of W
 
 // ---- TMEM columns ----------------------------------------------------------
 constexpr uint32_t TM_G = 0;     // lanes 64-127: G [i][j]
-constexpr uint32_t TM_DS = 64;   // W^T B [row][n], two buffers of 128 columns
-constexpr uint32_t TM_QS = 320;  // (C S)^T [row][i]
-constexpr uint32_t TM_PV = 384;  // (M X)^T [row][i]
-constexpr uint32_t TM_SB = 448;  // S as bf16 [row][n]: A operand
+constexpr uint32_t TM_DS = 64;   // W^T B [row][n] (STATE_ONLY: two buffers of 128 columns)
+constexpr uint32_t TM_QS = 192;  // (C S)^T [row][i], two buffers of 64 columns
+constexpr uint32_t TM_PV = 320;  // (M X)^T [row][i]
+constexpr uint32_t TM_SB = 384;  // S as bf16 [row][n]: A operand, two buffers of 64 columns
 constexpr uint32_t kTmemCols = 512;
 
 // ---- per-token tables (floats) of one head and chunk ------------------------
@@ -115,11 +117,11 @@ enum : int {
   B_BC = 0,                 // kStages: a chunk's B and C landed
   B_X = B_BC + kStages,     // kStages: its x landed and its tables are written
   B_EMPTY = B_X + kStages,  // kStages: every product that reads the stage is done
-  B_DONE = B_EMPTY + kStages,  // kStages: the compute warps are through with a chunk, and with the
-                               // state that the next one reads
-  B_START = B_DONE + kStages,  // the state that chunk 0 reads
-  B_RDY_W, B_RDY_M, B_RDY_D,   // compute warps -> issue warp
-  B_G, B_DS, B_DS1, B_PV, B_QS, B_END, kNumBars  // products done
+  B_DONE = B_EMPTY + kStages,  // kStages: the compute warps are through with a chunk
+  B_RDY_W = B_DONE + kStages, B_RDY_M,  // compute warps -> issue warp: operands of a chunk,
+  B_RDY_S, B_RDY_D,                     // the state it starts from, its accumulators read
+  // products done (two where a chunk's may complete before every warp has met the one before)
+  B_G, B_DS, B_DS1, B_PV, B_QS, B_QS1, B_END, kNumBars
 };
 static_assert(kNumBars * 8 + 12 <= 256, "barrier area");
 
@@ -210,8 +212,9 @@ struct Piece {
   int index, count;       // of the sequence's pieces
 };
 
-// The piece of slot `slot`: sequences in order, each with max(1, ceil(length / seg)) pieces.
-// Every warp finds it by itself, 32 sequences at a time.
+// The piece of slot `slot`: sequences in order, each with max(1, ceil(length / seg)) pieces,
+// less its last one with STATE_ONLY.  Every warp finds it by itself, 32 sequences at a time.
+template <bool STATE_ONLY>
 __device__ __forceinline__ Piece find_piece(const Params& p, int64_t slot) {
   const int lane = threadIdx.x & 31;
   Piece r{-1, 0, 0, 0, 1};
@@ -232,7 +235,7 @@ __device__ __forceinline__ Piece find_piece(const Params& p, int64_t slot) {
     int cnt = 0;
     if (n < p.N) {
       bounds(n, &b, &e);
-      cnt = static_cast<int>(max(int64_t(1), (e - b + p.seg - 1) / p.seg));
+      cnt = static_cast<int>(max(int64_t(1), (e - b + p.seg - 1) / p.seg)) - (STATE_ONLY ? 1 : 0);
     }
     int incl = cnt;
 #pragma unroll
@@ -246,8 +249,8 @@ __device__ __forceinline__ Piece find_piece(const Params& p, int64_t slot) {
       r.seq = base + src;
       b = __shfl_sync(0xffffffffu, b, src);
       e = __shfl_sync(0xffffffffu, e, src);
-      r.count = __shfl_sync(0xffffffffu, cnt, src);
-      r.index = static_cast<int>(slot - acc) - (__shfl_sync(0xffffffffu, incl, src) - r.count);
+      r.index = static_cast<int>(slot - acc) - __shfl_sync(0xffffffffu, incl - cnt, src);
+      r.count = __shfl_sync(0xffffffffu, cnt, src) + (STATE_ONLY ? 1 : 0);
       r.bos = b + r.index * p.seg;
       r.eos = min(r.bos + p.seg, e);
       return r;
@@ -286,8 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h0 = g * group_heads + (tile % group_tiles) * kHeads;  // first head of the tile
   const bool two = kHeads == 2 && h0 + 1 < (g + 1) * group_heads;  // its second head exists
 
-  const Piece pc = find_piece(p, slot);
-  if (pc.seq < 0 || (STATE_ONLY && pc.index == pc.count - 1)) return;
+  const Piece pc = find_piece<STATE_ONLY>(p, slot);
+  if (pc.seq < 0) return;
   const int64_t bos = pc.bos, Ltot = pc.eos - pc.bos;
   const bool last_piece = pc.index == pc.count - 1;
   const int n = static_cast<int>((Ltot + kChunk - 1) / kChunk);
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < kNumBars; ++i)
       mbar_init(&bars[i], i == B_RDY_W ? (STATE_ONLY ? kComputeWarps : 12) : i == B_RDY_M ? 6
-                         : (i == B_RDY_D || (i >= B_DONE && i <= B_START)) ? kComputeWarps
+                         : (i == B_RDY_S || i == B_RDY_D || (i >= B_DONE && i < B_DONE + kStages)) ? kComputeWarps
                          : i >= B_X && i < B_EMPTY ? 1 + kHeads : 1);
     fence_mbar_init();
     *abort_flag = 0u;
@@ -390,7 +393,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!STATE_ONLY) {
       for (int j = 0; j < pc.index; ++j) {  // through the pieces before this one
-        const int64_t u = (slot - pc.index + j) * p.tiles + tile;
+        // (the slot among the pieces that are not a sequence's last)
+        const int64_t u = (slot - pc.index - pc.seq + j) * p.tiles + tile;
         const float dec = p.ws_dec[2 * u + hh];
         const float4* F = reinterpret_cast<const float4*>(p.ws) + u * (kRows * NS / 4) + tid;
 #pragma unroll
@@ -403,20 +407,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    auto publish_state = [&]() {  // S as the bf16 A operand of (C S)^T
+    auto publish_state = [&](int c) {  // S at the start of chunk c as the bf16 A operand of (C S)^T
+      const uint32_t dst = tl + TM_SB + 64 * (c & 1);
       uint32_t w[kCols / 2];
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) w[i] = pack_bf16x2(s[2 * i], s[2 * i + 1]);
       if constexpr (kCols == 32)
-        tmem_st16u(tl + TM_SB + 16 * cq, w);
+        tmem_st16u(dst + 16 * cq, w);
       else
-        tmem_st8u(tl + TM_SB + 8 * cq, w);
+        tmem_st8u(dst + 8 * cq, w);
       tmem_wait_st();
+      signal(B_RDY_S, false);
     };
-    if (!STATE_ONLY) {
-      publish_state();
-      signal(B_START, false);
-    }
+    if (!STATE_ONLY) publish_state(0);
+    constexpr int kDsBufs = STATE_ONLY ? 2 : 1;
+    auto wait_ds = [&](int c) { wait(B_DS + c % kDsBufs, static_cast<uint32_t>((c / kDsBufs) & 1)); };
 
     // ---- W of chunk c, in 16-byte pieces of x (a warp takes two tokens at a time, a token on 16
     //      lanes).  The warps of quarters 0-1 take three such pairs, 16 tokens apart; the four
@@ -450,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               sts128(xs + L::kX + wblk * 8192 + k * (kStride * 128), 0u, 0u, 0u, 0u);
           }
       }
-      if (c > 0) wait(B_DS + ((c - 1) & 1), static_cast<uint32_t>(((c - 1) >> 1) & 1));  // W is free
+      if (c > 0) wait_ds(c - 1);  // W is free
       float2 chk = make_float2(0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < kCount; ++k) {
@@ -578,10 +583,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       float eg[16], qs[16], pv[16];
       load16(table(st, hh) + G_EG + 16 * cq, eg);
       if (quarter < 2 || (quarter == 2 && cq >= 2) || c + 1 == n) wait(B_PV, par);  // (the others waited for it to write M)
-      wait(B_QS, par);
+      wait(B_QS + (c & 1), static_cast<uint32_t>((c >> 1) & 1));
       const bool bad = *any_bad != 0u;  // (written before this chunk's W was signalled)
       tmem_ld16(tl + TM_PV + 16 * cq, pv);
-      tmem_ld16(tl + TM_QS + 16 * cq, qs);
+      tmem_ld16(tl + TM_QS + 64 * (c & 1) + 16 * cq, qs);
       tmem_wait_ld();
       reg_fence(pv);
       reg_fence(qs);
@@ -632,12 +637,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float dec = decs[st * 2 + hh];
       dprod *= dec;
       if (c + 1 == n || (!STATE_ONLY && !w_all && !w_some))  // (the others waited for it to write W)
-        wait(B_DS + (c & 1), static_cast<uint32_t>((c >> 1) & 1));
+        wait_ds(c);
       float v[kCols];
       if constexpr (kCols == 32)
-        tmem_ld32(tl + TM_DS + 128 * (c & 1) + 32 * cq, v);
+        tmem_ld32(tl + TM_DS + 128 * (c % kDsBufs) + 32 * cq, v);
       else
-        tmem_ld16(tl + TM_DS + 128 * (c & 1) + 16 * cq, v);
+        tmem_ld16(tl + TM_DS + 128 * (c % kDsBufs) + 16 * cq, v);
       tmem_wait_ld();
       reg_fence(v);
 #pragma unroll
@@ -646,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         s[i] = r.x;
         s[i + 1] = r.y;
       }
-      if (!STATE_ONLY && c + 1 < n) publish_state();
+      if (!STATE_ONLY && c + 1 < n) publish_state(c + 1);
     };
 
     // (buffer and stage of chunk c + 1, and their parity)
@@ -673,8 +678,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (c >= 0) {
-        if (!STATE_ONLY) outputs(c, prev);
         update(c, prev);
+        if (!STATE_ONLY) outputs(c, prev);
         signal(B_DONE + prev, !STATE_ONLY);
       }
       prev = st;
@@ -726,14 +731,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
     auto mma_ds = [&](int c, int st) {
-      const uint32_t d = tm + TM_DS + 128 * (c & 1), bc = sb16 + kBc16 + st * kStage16;
+      const uint32_t d = tm + TM_DS + (STATE_ONLY ? 128 * (c & 1) : 0), bc = sb16 + kBc16 + st * kStage16;
 #pragma unroll
       for (int part = 0; part < kTerms; ++part)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
           mma_ss_by(leader, d, sdesc_sw128_f(sb16 + (L::OFF_W + part * 16384 + ks * 2048) / 16, 8192, 1024),
                     sdesc_sw128_f(bc + ks * 128, 16384, 1024), idesc_ds, part > 0 || ks > 0);
-      commit_by(leader, &bars[B_DS + (c & 1)]);
+      commit_by(leader, &bars[B_DS + (STATE_ONLY ? c & 1 : 0)]);
     };
     auto mma_pv = [&](int st) {
       const uint32_t xo = L::OFF_ST + st * L::kStage;
@@ -754,13 +759,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       commit_by(leader, &bars[B_PV]);
     };
-    auto mma_qs = [&](int st) {
+    auto mma_qs = [&](int c, int st) {
       const uint32_t bc = sb16 + kBc16 + st * kStage16;
 #pragma unroll
       for (int ks = 0; ks < NS / 16; ++ks)
-        mma_ts_by(leader, tm + TM_QS, tm + TM_SB + 8 * ks,
+        mma_ts_by(leader, tm + TM_QS + 64 * (c & 1), tm + TM_SB + 64 * (c & 1) + 8 * ks,
                   sdesc_sw128_f(bc + ((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) / 16, 16, 1024), idesc_qs, ks > 0);
-      commit_by(leader, &bars[B_QS]);
+      commit_by(leader, &bars[B_QS + (c & 1)]);
     };
     bool ok = STATE_ONLY || mma_g(0, 0);
     // stages of chunks c, c + 1 and c + 2, and the parities of c's and of c + 2's
@@ -768,27 +773,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t par0 = 1, par2 = 0;
     for (int c = -1; ok && c < n; ++c) {
       const uint32_t next = static_cast<uint32_t>((c + 1) & 1);
-      if (c + 1 < n) {
-        // (its buffer's readers, the update of chunk c - 1, are done: B_DONE below; with
-        // STATE_ONLY here)
-        if (STATE_ONLY && c >= 1 && !(ok = wait(B_DONE + (c - 1) % kStages, static_cast<uint32_t>(((c - 1) / kStages) & 1))))
-          break;
-        if (STATE_ONLY && !(ok = wait(B_BC + s1, s1 == 0 ? par0 ^ 1u : par0))) break;
+      if (STATE_ONLY) {
+        if (c + 1 == n) break;
+        // (the buffer of W^T B was read in the update of chunk c - 1)
+        if (c >= 1 && !(ok = wait(B_DONE + (c - 1) % kStages, static_cast<uint32_t>(((c - 1) / kStages) & 1)))) break;
+        if (!(ok = wait(B_BC + s1, s1 == 0 ? par0 ^ 1u : par0))) break;
         if (!(ok = wait(B_RDY_W, next))) break;
         mma_ds(c + 1, s1);
-        if (STATE_ONLY) {
-          commit_by(leader, &bars[B_EMPTY + s1]);
-        } else {
+        commit_by(leader, &bars[B_EMPTY + s1]);
+      } else {
+        if (c + 1 < n) {
           if (!(ok = wait(B_RDY_M, next))) break;
           if (c + 2 < n && !(ok = mma_g(s2, par2))) break;
+          if (!(ok = wait(B_RDY_W, next))) break;
+          if (!(ok = wait(B_RDY_S, next))) break;  // the update of chunk c has read W^T B
+          mma_ds(c + 1, s1);
+          mma_qs(c + 1, s1);
         }
-      }
-      if (!STATE_ONLY) {
-        if (c >= 0 && !(ok = wait(B_RDY_D, next ^ 1u))) break;  // the outputs of chunk c left their accumulators
+        if (c >= 0 && !(ok = wait(B_RDY_D, next ^ 1u))) break;  // the outputs of chunk c have read their accumulators
         if (c + 1 < n) {
           mma_pv(s1);
-          if (!(ok = c < 0 ? wait(B_START, 0) : wait(B_DONE + s0, par0))) break;
-          mma_qs(s1);
           commit_by(leader, &bars[B_EMPTY + s1]);
         }
       }
@@ -1008,9 +1012,38 @@ struct Cut {
   int64_t slots = 0;  // at most so many pieces
 };
 
+// Times in units of one chunk of the second launch on one SM (~2.6 us): a chunk of the first,
+// the start and end of a CTA, the state of one earlier piece, a launch.
+constexpr double kStateChunk = 0.4, kCta = 3.0, kJoin = 0.3, kLaunch = 1.5;
+
+// Only the mean length is known here (the lengths lie on the device): the piece length is the
+// one that is best for sequences of that length.  Calls that fill the SMs with whole sequences
+// are cut too, but only sequences of twice the work of an SM: one long sequence among short
+// ones would run on alone for most of the call.
 Cut choose_cut(int64_t T, int64_t N, int64_t tiles, int sms) {
-  (void)sms, (void)tiles, (void)T;
-  return Cut{0, N};
+  const int64_t chunks = std::max<int64_t>(1, (T + N * kChunk - 1) / (N * kChunk));  // of a mean sequence
+  auto waves = [&](int64_t ctas) { return static_cast<double>((ctas + sms - 1) / sms); };
+  Cut best{0, N};
+  double best_time = waves(N * tiles) * (chunks + kCta);
+  for (int64_t p = 2; p <= 64 && p <= chunks; ++p) {
+    const int64_t seg = (chunks + p - 1) / p;
+    if (seg < 2) break;
+    const int64_t pieces = (chunks + seg - 1) / seg;
+    const double time = waves(N * (pieces - 1) * tiles) * (seg * kStateChunk + kCta) + kLaunch +
+                        waves(N * pieces * tiles) * (seg + kCta + kJoin * (pieces - 1) / 2);
+    if (time < 0.9 * best_time) {
+      best_time = time;
+      best.seg = seg;
+    }
+  }
+  const int64_t all = T / kChunk, share = (all * tiles + sms - 1) / sms;  // chunks of an SM, were they spread evenly
+  const int64_t longest = std::max(2 * share, chunks + 1);
+  if (best.seg == 0 && all >= 64 && 2 * longest <= all) best.seg = longest;
+  if (best.seg) {
+    best.seg *= kChunk;
+    best.slots = N + T / best.seg;  // the pieces of N sequences of T tokens are at most this many
+  }
+  return best;
 }
 
 template <int P, int NS, bool STATE_ONLY>
@@ -1037,8 +1070,9 @@ cudaError_t launch(const SsmArgs& a, const Cut& cut, void* ws, cudaStream_t s) {
            static_cast<__nv_bfloat16*>(a.out), a.new_state, static_cast<float*>(ws), nullptr, a.T, a.N, cut.seg,
            static_cast<int>(a.H), static_cast<int>(a.G), static_cast<int>(head_tiles(a.H, a.G, P))};
   if (cut.seg) {
-    p.ws_dec = p.ws + cut.slots * p.tiles * kRows * NS;
-    if ((e = launch_one<P, NS, true>(m, p, cut.slots, s)) != cudaSuccess) return e;
+    const int64_t inner = cut.slots - a.N;  // pieces that are not a sequence's last
+    p.ws_dec = p.ws + inner * p.tiles * kRows * NS;
+    if (inner > 0 && (e = launch_one<P, NS, true>(m, p, inner, s)) != cudaSuccess) return e;
   }
   return launch_one<P, NS, false>(m, p, cut.slots, s);
 }
@@ -1048,7 +1082,7 @@ cudaError_t launch(const SsmArgs& a, const Cut& cut, void* ws, cudaStream_t s) {
 size_t ssm_chunked_workspace(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P, int64_t Ns, int sms) {
   const int64_t tiles = head_tiles(H, G, P);
   const Cut cut = choose_cut(T, N, tiles, sms);
-  return cut.seg ? static_cast<size_t>(cut.slots) * tiles * (kRows * Ns + 2) * sizeof(float) : 0;
+  return cut.seg ? static_cast<size_t>(cut.slots - N) * tiles * (kRows * Ns + 2) * sizeof(float) : 0;
 }
 
 cudaError_t launch_ssm_chunked(const SsmArgs& a, void* ws, int sms, cudaStream_t s) {

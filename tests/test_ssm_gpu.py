@@ -231,3 +231,38 @@ def test_same_answer_twice_and_beside_other_sequences():
     assert torch.equal(y, y2) and torch.equal(s, s2)
     y3, s3 = run(300, 365, st[1:2], torch.tensor([0, 65], device="cuda"))
     assert torch.equal(y[300:365], y3) and torch.equal(s[1:2], s3)
+
+
+@pytest.mark.parametrize("H,P,G,Ns,lens,state", [
+    (2, 64, 1, 128, [1900], True),               # few pairs: pieces of a few chunks
+    (2, 128, 2, 64, [3300, 0, 2700, 5], True),
+    (3, 64, 1, 64, [2048 + 33], False),
+    (4, 64, 1, 128, [64 * 32, 64 * 30 + 1], True),  # a last piece of one token
+])
+def test_sequences_cut_into_pieces(H, P, G, Ns, lens, state):
+    """Calls of few (sequence, head) pairs, whose sequences run as pieces joined by their decays."""
+    from gdn_b200 import ssm
+    assert ssm.workspace_bytes(sum(lens), len(lens), H, G, P, Ns) > 0
+    m = make((sum(lens),), H, P, G, Ns, seed=sum(lens))
+    st = torch.randn(len(lens), H, P, Ns, device="cuda") if state else None
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0)
+    out, new = ssm.run(m["x"], m["B"], m["C"], st, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)
+    check_packed(m, lens, st, out, new)
+
+
+def test_one_long_sequence_among_many():
+    """A batch that fills the GPU, one of whose sequences is long enough to be cut."""
+    from gdn_b200 import ssm
+    lens = [40] * 70 + [9000] + [33] * 40
+    H, G = 8, 1
+    assert ssm.workspace_bytes(sum(lens), len(lens), H, G, 64, 128) > 0
+    m = make((sum(lens),), H, 64, G, 128, seed=2)
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0)
+    out, new = ssm.run(m["x"], m["B"], m["C"], None, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)
+    # the sequences on both sides, and the whole long one
+    for i in (0, 69, 70, 71, 110):
+        a, b = int(cu[i]), int(cu[i + 1])
+        y, ya, S, Sa = L.scan_ref(*(m[k][a:b] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"],
+                                  torch.zeros(H, 64, 128))
+        L.within(out[a:b], y, y_slack(ya, b - a))
+        L.within(new[i], S, s_slack(Sa, b - a))
