@@ -8,11 +8,16 @@
 // ([.., H, P, Ns]); head h reads B and C of group h / (H / G).
 //
 // Bound by the state's bytes (single tokens: 8 bytes an element in fp32 against ~4
-// operations).  A warp owns kRows rows of one head; the lanes of a row hold 16 bytes of
-// it each, so a warp's load covers whole 128-byte lines, and all of a warp's rows are in
-// flight before the first is used.  The rows' dot products with C are reduced
-// together: each exchange halves the values a lane still sums (9 shuffles for 8 rows
-// instead of 40).  State and sums are fp32; a bf16 pool is rounded once per store.
+// operations).  A warp owns a batch of rows of one head; the lanes of a row hold 16 bytes of it
+// each, so a warp's load covers whole 128-byte lines, and all of the batch's loads are in
+// flight before the first is used.  The rows' dot products with C are reduced together: each
+// exchange halves the values a lane still sums (9 shuffles for 8 rows instead of 40).  Gates
+// are computed a token on a lane.  State and sums are fp32; a bf16 pool is rounded once per
+// store.  Single tokens have their own instantiation, whose rows go from the raw load to the
+// store one by one; with several, the rows stay in registers and four tokens' sums are reduced at
+// once.  Measured with states larger than L2: single tokens, fp32, 256 x 64 heads of 64 x 128,
+// 161 us (1.02 of the copy peak; 174 with two blocks per SM instead of three); bf16 84 us (0.99;
+// 90 with three).  Four tokens, where the arithmetic counts: fp32 0.70, bf16 0.46.
 #include "gdn_internal.h"
 #include "gdn_vec16.cuh"
 
@@ -20,73 +25,100 @@ namespace gdn {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kU = 8;  // rows a lane holds a part of
 
-
-template <bool BF16, int kVec>
-__device__ __forceinline__ void load_state(const void* base, int64_t elem, float* s) {
+// 16 bytes of state as loaded: four fp32 or eight bf16 elements
+template <bool BF16>
+__device__ __forceinline__ uint4 load_state(const void* base, int64_t elem) {
+  return ld_cs_u4(static_cast<const uint8_t*>(base) + elem * (BF16 ? 2 : 4));
+}
+template <bool BF16>
+__device__ __forceinline__ void widen(uint4 w, float2 (&s)[BF16 ? 4 : 2]) {
   if constexpr (BF16) {
-    unpack8<Bf16>(ld_cs_u4(static_cast<const uint16_t*>(base) + elem), s);
+    s[0] = Bf16::unpack(w.x);
+    s[1] = Bf16::unpack(w.y);
+    s[2] = Bf16::unpack(w.z);
+    s[3] = Bf16::unpack(w.w);
   } else {
-    const float4 v = ld_stream_f4(static_cast<const float*>(base) + elem);
-    s[0] = v.x;
-    s[1] = v.y;
-    s[2] = v.z;
-    s[3] = v.w;
+    s[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+    s[1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
   }
 }
-
-template <bool BF16, int kVec>
-__device__ __forceinline__ void store_state(void* base, int64_t elem, const float* s) {
-  if constexpr (BF16) {
-    const uint4 v = pack8<Bf16>(s);
-    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(static_cast<uint16_t*>(base) + elem),
-                 "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                 : "memory");
-  } else {
-    st_stream_f4(static_cast<float*>(base) + elem, make_float4(s[0], s[1], s[2], s[3]));
-  }
-}
-
-// kVec consecutive bf16 values (8 or 16 bytes), widened
-template <int kVec>
-__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float* v) {
-  if constexpr (kVec == 8)
-    unpack8<Bf16>(ldg_u4(p), v);
+template <bool BF16>
+__device__ __forceinline__ void store_state(void* base, int64_t elem, const float2 (&s)[BF16 ? 4 : 2]) {
+  uint4 v;
+  if constexpr (BF16)
+    v = make_uint4(pack_bf16x2(s[0].x, s[0].y), pack_bf16x2(s[1].x, s[1].y), pack_bf16x2(s[2].x, s[2].y),
+                   pack_bf16x2(s[3].x, s[3].y));
   else
-    ld_bf16x4(p, v);
+    v = make_uint4(__float_as_uint(s[0].x), __float_as_uint(s[0].y), __float_as_uint(s[1].x), __float_as_uint(s[1].y));
+  asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(static_cast<uint8_t*>(base) + elem * (BF16 ? 2 : 4)),
+               "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+// A lane's part of a B or C row (eight or four bf16), raw and widened
+template <int kPairs>
+struct Vec;
+template <>
+struct Vec<2> {
+  uint2 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  }
+  __device__ __forceinline__ void widen(float2 (&f)[2]) const {
+    f[0] = Bf16::unpack(v.x);
+    f[1] = Bf16::unpack(v.y);
+  }
+};
+template <>
+struct Vec<4> {
+  uint4 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = ldg_u4(p); }
+  __device__ __forceinline__ void widen(float2 (&f)[4]) const {
+    f[0] = Bf16::unpack(v.x);
+    f[1] = Bf16::unpack(v.y);
+    f[2] = Bf16::unpack(v.z);
+    f[3] = Bf16::unpack(v.w);
+  }
+};
+
+// kN bf16 values, kN = 4 or 8, widened
+template <int kN>
+__device__ __forceinline__ void widen_x(const Vec<kN / 2>& v, float (&x)[kN]) {
+  float2 f[kN / 2];
+  v.widen(f);
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    x[2 * i] = f[i].x;
+    x[2 * i + 1] = f[i].y;
+  }
 }
 
 // Ns = 64 or 128; BF16: storage of the state; PACKED: prompts by cu_seqlens (fp32 states
-// in and out) instead of a pool.
-template <int Ns, bool BF16, bool PACKED>
-__global__ void __launch_bounds__(kWarps * 32) gdn_ssm_recurrent_kernel(SsmArgs p) {
-  constexpr int kVec = BF16 ? 8 : 4;
+// in and out) instead of a pool; ONE: a single token of each sequence; kU: rows a lane holds a
+// part of.
+template <int Ns, bool BF16, bool PACKED, bool ONE, int kU, int kBlocks>
+__global__ void __launch_bounds__(kWarps * 32, kBlocks) gdn_ssm_recurrent_kernel(SsmArgs p) {
+  constexpr int kVec = BF16 ? 8 : 4, kPairs = kVec / 2;
   constexpr int kLanes = Ns / kVec;        // lanes of a row: 8, 16 or 32
-  constexpr int kPar = 32 / kLanes;        // rows of one warp access
-  constexpr int kRows = kU * kPar;         // rows of a warp: 8, 16 or 32
+  constexpr int kRows = kU * 32 / kLanes;  // rows of a warp
   const int lane = threadIdx.x & 31;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t per_head = p.P / kRows;    // P is 64 or 128: a multiple of kRows
-  const int64_t n = unit / (p.H * per_head);
+  const int per_head = static_cast<int>(p.P) / kRows;  // P is 64 or 128: a multiple of kRows
+  const int64_t nh = unit / per_head;
+  const int64_t n = nh / p.H;
   if (n >= p.N) return;
-  const int64_t hr = unit - n * p.H * per_head;
-  const int64_t h = hr / per_head;
-  const int64_t row0 = (hr - h * per_head) * kRows + lane / kLanes;  // + kPar u
-  const int64_t g = h / (p.H / p.G);
+  const int h = static_cast<int>(nh - n * p.H);
+  const int row0 = static_cast<int>(unit - nh * per_head) * kRows + lane / kLanes * kU;  // this lane's first row
+  const int g = h / static_cast<int>(p.H / p.G);
   const int col = (lane % kLanes) * kVec;
 
-  const __nv_bfloat16* xs = static_cast<const __nv_bfloat16*>(p.x);
-  const __nv_bfloat16* bs = static_cast<const __nv_bfloat16*>(p.B);
-  const __nv_bfloat16* cs = static_cast<const __nv_bfloat16*>(p.C);
-  const __nv_bfloat16* as = static_cast<const __nv_bfloat16*>(p.a);
-  __nv_bfloat16* ys = static_cast<__nv_bfloat16*>(p.out);
-
-  int64_t tok = 0, len = p.T;  // first token (a row of x, B, C, a, y) and their number
+  int64_t tok = 0;  // first token (a row of x, B, C, a, y) and their number
+  int len = static_cast<int>(p.T);
   int64_t in = n, outs = n;
   if constexpr (PACKED) {
     tok = min(max(p.cu_seqlens[n], int64_t(0)), p.T);
-    len = min(max(p.cu_seqlens[n + 1], tok), p.T) - tok;
+    len = static_cast<int>(min(max(p.cu_seqlens[n + 1], tok), p.T) - tok);
   } else {
     tok = n * p.T;
     in = p.in_slots[n];
@@ -96,51 +128,56 @@ __global__ void __launch_bounds__(kWarps * 32) gdn_ssm_recurrent_kernel(SsmArgs 
   const bool has_out = PACKED || (!p.no_state_update && outs >= 0 && outs < p.pool_size);
   const void* src = PACKED ? static_cast<const void*>(p.state) : p.pool;
   void* dst = PACKED ? static_cast<void*>(p.new_state) : p.pool;
+  const int64_t src0 = ((in * p.H + h) * p.P + row0) * Ns + col;
+  const int64_t dst0 = ((outs * p.H + h) * p.P + row0) * Ns + col;
 
-  float s[kU][kVec];
+  uint4 raw[kU];
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    if (has_in)
-      load_state<BF16, kVec>(src, ((in * p.H + h) * p.P + row0 + kPar * u) * Ns + col, s[u]);
-    else
+  for (int u = 0; u < kU; ++u) raw[u] = has_in ? load_state<BF16>(src, src0 + u * Ns) : make_uint4(0, 0, 0, 0);
+
+  const __nv_bfloat16* xs = static_cast<const __nv_bfloat16*>(p.x) + (tok * p.H + h) * p.P + row0;
+  const __nv_bfloat16* bs = static_cast<const __nv_bfloat16*>(p.B) + (tok * p.G + g) * Ns + col;
+  const __nv_bfloat16* cs = static_cast<const __nv_bfloat16*>(p.C) + (tok * p.G + g) * Ns + col;
+  const __nv_bfloat16* as = static_cast<const __nv_bfloat16*>(p.a) + tok * p.H + h;
+  __nv_bfloat16* ys = static_cast<__nv_bfloat16*>(p.out) + (tok * p.H + h) * p.P + row0;
+  const int64_t xpitch = p.H * p.P, bpitch = p.G * Ns;
+
+  // kTok tokens at a time: their inputs are loaded together, and their dot products reduced together
+  constexpr int kTok = ONE ? 1 : 4;
+  Vec<kPairs> Bn[kTok], Cn[kTok];
+  Vec<kU / 2> xn[kTok];
+  auto inputs = [&](int t0) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) s[u][e] = 0.f;
-  }
+    for (int i = 0; i < kTok; ++i) {
+      const int64_t t = ONE ? 0 : min(t0 + i, len - 1);
+      Bn[i].load(bs + t * bpitch);
+      Cn[i].load(cs + t * bpitch);
+      xn[i].load(xs + t * xpitch);
+    }
+  };
+  if (ONE || len > 0) inputs(0);
   const float negA = -expf(p.A_log[h]);
   const float bias = p.dt_bias[h];
   const float skip = p.D ? p.D[h] : 0.f;
-  // after the reduction lane l holds the sum of row kPar u + (its row group), u from
-  // the lane bits that the exchanges below consumed
-  const int ur = kLanes == 32 ? (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1)
-                 : kLanes == 16 ? (lane >> 3 & 1) * 4 + (lane >> 2 & 1) * 2 + (lane >> 1 & 1)
-                                : (lane >> 2 & 1) * 4 + (lane >> 1 & 1) * 2 + (lane & 1);
-  constexpr int kSpare = kLanes / 8 - 1;  // lanes of the same row beyond the first
-  const bool writer = (lane & kSpare) == 0;
-
-  for (int64_t t = 0; t < len; ++t) {
-    const int64_t r = tok + t;
-    float B[kVec], C[kVec];
-    load_vec<kVec>(bs + (r * p.G + g) * Ns + col, B);
-    load_vec<kVec>(cs + (r * p.G + g) * Ns + col, C);
-    const float dt = softplus_t20(__bfloat162float(as[r * p.H + h]) + bias);
-    const float dec = expf(negA * dt);
-    const __nv_bfloat16* xrow = xs + (r * p.H + h) * p.P + row0;
-    float xv[kU];
+  float dts = 0.f, decs = 0.f;  // of token (t & ~31) + lane; with ONE of token 0
+  auto gates = [&](int t) {
+    dts = softplus_t20(__bfloat162float(as[t * p.H]) + bias);
+    decs = expf(negA * dts);
+  };
+  if (ONE)
+    gates(0);
+  else if (lane < len)
+    gates(lane);
+  // Sums of kTok x kU values over the lanes of a row: every exchange halves the values that a
+  // lane still sums; it ends with kLeft of them, the first of which is number `mine`.
+  constexpr int kVals = kTok * kU, kLeft = kVals > kLanes ? kVals / kLanes : 1;
+  int mine = 0;
 #pragma unroll
-    for (int u = 0; u < kU; ++u) xv[u] = __bfloat162float(xrow[kPar * u]);
-    float acc[kU];
+  for (int half = kVals / 2, bit = kLanes / 2; half >= kLeft && bit >= 1; half >>= 1, bit >>= 1) mine |= lane & bit ? half : 0;
+  const bool writer = kVals >= kLanes || (lane & (kLanes / kVals - 1)) == 0;
+  auto reduce_and_write = [&](float (&acc)[kVals], int t0) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const float w = dt * xv[u];
-      acc[u] = 0.f;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        s[u][e] = fmaf(dec, s[u][e], w * B[e]);
-        acc[u] = fmaf(s[u][e], C[e], acc[u]);
-      }
-    }
-#pragma unroll
-    for (int half = kU / 2, bit = kLanes / 2; half >= 1; half >>= 1, bit >>= 1) {
+    for (int half = kVals / 2, bit = kLanes / 2; half >= kLeft && bit >= 1; half >>= 1, bit >>= 1) {
       const bool up = lane & bit;
 #pragma unroll
       for (int u = 0; u < half; ++u) {
@@ -150,37 +187,97 @@ __global__ void __launch_bounds__(kWarps * 32) gdn_ssm_recurrent_kernel(SsmArgs 
       }
     }
 #pragma unroll
-    for (int bit = kLanes / 16; bit >= 1; bit >>= 1)
-      acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], bit);
-    float xo = xv[0];
+    for (int bit = kLanes / kVals / 2; bit >= 1; bit >>= 1) acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], bit);
 #pragma unroll
-    for (int u = 1; u < kU; ++u) xo = ur == u ? xv[u] : xo;
-    if (writer)
-      ys[(r * p.H + h) * p.P + row0 + kPar * ur] = __float2bfloat16_rn(fmaf(skip, xo, acc[0]));
-  }
-  if (has_out) {
+    for (int i = 0; i < kLeft; ++i) {
+      const int64_t at = (t0 + (mine + i) / kU) * xpitch + (mine + i) % kU;
+      if (writer && (ONE || t0 + (mine + i) / kU < len))
+        ys[at] = __float2bfloat16_rn(fmaf(skip, __bfloat162float(xs[at]), acc[i]));
+    }
+  };
+  // one row's step: s <- dec s + w B; returns s . C over this lane's elements
+  auto step = [&](float2 (&s)[kPairs], float w, float dec, const float2 (&B)[kPairs], const float2 (&C)[kPairs]) {
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
-      store_state<BF16, kVec>(dst, ((outs * p.H + h) * p.P + row0 + kPar * u) * Ns + col, s[u]);
+    for (int e = 0; e < kPairs; ++e) {
+      s[e] = __ffma2_rn(make_float2(dec, dec), s[e], __fmul2_rn(make_float2(w, w), B[e]));
+      sum = __ffma2_rn(s[e], C[e], sum);
+    }
+    return sum.x + sum.y;
+  };
+
+  float acc[kVals];
+  if constexpr (ONE) {
+    float2 B[kPairs], C[kPairs];
+    float xv[kU];
+    Bn[0].widen(B);
+    Cn[0].widen(C);
+    widen_x<kU>(xn[0], xv);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float2 s[kPairs];
+      widen<BF16>(raw[u], s);
+      acc[u] = step(s, dts * xv[u], decs, B, C);
+      if (has_out) store_state<BF16>(dst, dst0 + u * Ns, s);
+    }
+    reduce_and_write(acc, 0);
+  } else {
+    float2 s[kU][kPairs];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) widen<BF16>(raw[u], s[u]);
+#pragma unroll 1
+    for (int t0 = 0; t0 < len; t0 += kTok) {
+      if (t0 > 0) {
+        if ((t0 & 31) == 0 && t0 + lane < len) gates(t0 + lane);
+        inputs(t0);
+      }
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        if (t0 + i < len) {
+          const float dt = __shfl_sync(0xffffffffu, dts, (t0 + i) & 31), dec = __shfl_sync(0xffffffffu, decs, (t0 + i) & 31);
+          float2 B[kPairs], C[kPairs];
+          float xv[kU];
+          Bn[i].widen(B);
+          Cn[i].widen(C);
+          widen_x<kU>(xn[i], xv);
+#pragma unroll
+          for (int u = 0; u < kU; ++u) acc[i * kU + u] = step(s[u], dt * xv[u], dec, B, C);
+        } else {
+#pragma unroll
+          for (int u = 0; u < kU; ++u) acc[i * kU + u] = 0.f;
+        }
+      }
+      reduce_and_write(acc, t0);
+    }
+    if (has_out) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) store_state<BF16>(dst, dst0 + u * Ns, s[u]);
+    }
   }
 }
 
-template <int Ns, bool BF16, bool PACKED>
+template <int Ns, bool BF16, bool PACKED, bool ONE, int kU, int kBlocks>
 cudaError_t launch(const SsmArgs& a, cudaStream_t s) {
   constexpr int kRows = kU * 32 / (Ns / (BF16 ? 8 : 4));
   const int64_t units = a.N * a.H * (a.P / kRows);
   const int64_t blocks = (units + kWarps - 1) / kWarps;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  gdn_ssm_recurrent_kernel<Ns, BF16, PACKED><<<static_cast<unsigned>(blocks), kWarps * 32, 0, s>>>(a);
+  gdn_ssm_recurrent_kernel<Ns, BF16, PACKED, ONE, kU, kBlocks><<<static_cast<unsigned>(blocks), kWarps * 32, 0, s>>>(a);
   return cudaGetLastError();
+}
+
+// (blocks per SM as measured: see above)
+template <int Ns>
+cudaError_t by_form(const SsmArgs& a, cudaStream_t s) {
+  if (!a.in_slots) return launch<Ns, false, true, false, 8, 2>(a, s);
+  if (a.T == 1) return a.state_bf16 ? launch<Ns, true, false, true, 8, 2>(a, s) : launch<Ns, false, false, true, 8, 3>(a, s);
+  return a.state_bf16 ? launch<Ns, true, false, false, 8, 2>(a, s) : launch<Ns, false, false, false, 8, 2>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_ssm_recurrent(const SsmArgs& a, cudaStream_t s) {
-  if (!a.in_slots) return a.Ns == 64 ? launch<64, false, true>(a, s) : launch<128, false, true>(a, s);
-  if (a.state_bf16) return a.Ns == 64 ? launch<64, true, false>(a, s) : launch<128, true, false>(a, s);
-  return a.Ns == 64 ? launch<64, false, false>(a, s) : launch<128, false, false>(a, s);
+  return a.Ns == 64 ? by_form<64>(a, s) : by_form<128>(a, s);
 }
 
 }  // namespace gdn
