@@ -74,8 +74,8 @@ constexpr int kTerms = 3;   // bf16 terms of W
 constexpr uint32_t TM_G = 0;     // lanes 64-127: G [i][j]
 constexpr uint32_t TM_DS = 64;   // W^T B [row][n] (STATE_ONLY: two buffers of 128 columns)
 constexpr uint32_t TM_QS = 192;  // (C S)^T [row][i], two buffers of 64 columns
-constexpr uint32_t TM_PV = 320;  // (M X)^T [row][i]
-constexpr uint32_t TM_SB = 384;  // S as bf16 [row][n]: A operand, two buffers of 64 columns
+constexpr uint32_t TM_PV = 320;  // (M X)^T [row][i], two buffers of 64 columns
+constexpr uint32_t TM_SB = 448;  // S as bf16 [row][n]: A operand
 constexpr uint32_t kTmemCols = 512;
 
 // ---- per-token tables (floats) of one head and chunk ------------------------
@@ -119,9 +119,9 @@ enum : int {
   B_EMPTY = B_X + kStages,  // kStages: every product that reads the stage is done
   B_DONE = B_EMPTY + kStages,  // kStages: the compute warps are through with a chunk
   B_RDY_W = B_DONE + kStages, B_RDY_M,  // compute warps -> issue warp: operands of a chunk,
-  B_RDY_S, B_RDY_D,                     // the state it starts from, its accumulators read
+  B_RDY_S, B_RDY_D, B_RDY_D1,           // the state it starts from, its accumulators read
   // products done (two where a chunk's may complete before every warp has met the one before)
-  B_G, B_DS, B_DS1, B_PV, B_QS, B_QS1, B_END, kNumBars
+  B_G, B_DS, B_DS1, B_PV, B_PV1, B_QS, B_QS1, B_END, kNumBars
 };
 static_assert(kNumBars * 8 + 12 <= 256, "barrier area");
 
@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kNumBars; ++i)
-      mbar_init(&bars[i], i == B_RDY_W ? (STATE_ONLY ? kComputeWarps : 12) : i == B_RDY_M ? 6
-                         : (i == B_RDY_S || i == B_RDY_D || (i >= B_DONE && i < B_DONE + kStages)) ? kComputeWarps
+      mbar_init(&bars[i], i == B_RDY_W ? (STATE_ONLY ? kComputeWarps : kComputeWarps / 2) : i == B_RDY_M ? (kHeads == 2 ? 8 : 6)
+                         : (i == B_RDY_S || i == B_RDY_D || i == B_RDY_D1 || (i >= B_DONE && i < B_DONE + kStages)) ? kComputeWarps
                          : i >= B_X && i < B_EMPTY ? 1 + kHeads : 1);
     fence_mbar_init();
     *abort_flag = 0u;
@@ -407,8 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    auto publish_state = [&](int c) {  // S at the start of chunk c as the bf16 A operand of (C S)^T
-      const uint32_t dst = tl + TM_SB + 64 * (c & 1);
+    auto publish_state = [&]() {  // S as the bf16 A operand of (C S)^T
+      const uint32_t dst = tl + TM_SB;
       uint32_t w[kCols / 2];
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) w[i] = pack_bf16x2(s[2 * i], s[2 * i + 1]);
@@ -419,21 +419,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_st();
       signal(B_RDY_S, false);
     };
-    if (!STATE_ONLY) publish_state(0);
+    if (!STATE_ONLY) publish_state();
+    // products that come in two buffers by the chunk's parity
+    auto wait2 = [&](int b, int c) { wait(b + (c & 1), static_cast<uint32_t>((c >> 1) & 1)); };
     constexpr int kDsBufs = STATE_ONLY ? 2 : 1;
     auto wait_ds = [&](int c) { wait(B_DS + c % kDsBufs, static_cast<uint32_t>((c / kDsBufs) & 1)); };
 
-    // ---- W of chunk c, in 16-byte pieces of x (a warp takes two tokens at a time, a token on 16
-    //      lanes).  The warps of quarters 0-1 take three such pairs, 16 tokens apart; the four
-    //      whose part of M is above or below the diagonal two, 8 apart; those on the diagonal
-    //      none.  (STATE_ONLY: two each, 32 apart.) -----------------------------------
-    const bool w_all = quarter < 2, w_some = (quarter == 2 && cq >= 2) || (quarter == 3 && cq < 2);
-    const int wt = (STATE_ONLY ? 2 * warp : w_all ? (warp >> 2) * 4 + (warp & 1) * 2 : 48 + 2 * ((quarter & 1) * 2 + (cq & 1))) +
-                   (lane >> 4);
+    // ---- W of chunk c by quarters 0-1, in 16-byte pieces of x: a warp takes two tokens at a
+    //      time (a token on 16 lanes), four times, 16 tokens apart.  (STATE_ONLY: every warp, twice,
+    //      32 apart.)  Shares of it for quarters 2-3 delayed M and cost 5-20 %. -----------------
+    const bool has_w = STATE_ONLY || quarter < 2;
+    const int wt = (STATE_ONLY ? 2 * warp : (warp >> 2) * 4 + (warp & 1) * 2) + (lane >> 4);
     const int wblk = (lane >> 3) & 1;
     const uint32_t woff = wblk * 8192 + sw128_off(wt, lane & 7);
-    auto make_w = [&](auto stride, auto count, int c, int st, uint32_t st_par) {
-      constexpr int kStride = decltype(stride)::value, kCount = decltype(count)::value;
+    constexpr int kStride = STATE_ONLY ? 32 : 16, kCount = kChunk / kStride;
+    auto make_w = [&](int c, int st, uint32_t st_par) {
       const uint32_t xs = sb + L::OFF_ST + st * L::kStage + woff;
       const int Lc = static_cast<int>(min(static_cast<int64_t>(kChunk), Ltot - static_cast<int64_t>(c) * kChunk));
       wait(B_X + st, st_par);
@@ -457,26 +457,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (c > 0) wait_ds(c - 1);  // W is free
       float2 chk = make_float2(0.f, 0.f);
+      float2 v[kCount][4];
 #pragma unroll
       for (int k = 0; k < kCount; ++k) {
         const uint32_t xw[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-        float2 v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          v[e] = __fmul2_rn(make_float2(bf16_lo(xw[e]), bf16_hi(xw[e])), make_float2(w[k], w[k]));
+          v[k][e] = __fmul2_rn(make_float2(bf16_lo(xw[e]), bf16_hi(xw[e])), make_float2(w[k], w[k]));
+      }
 #pragma unroll
-        for (int term = 0; term < kTerms; ++term) {  // the rounded value, then what it left
-          uint32_t b[4];
+      for (int term = 0; term < kTerms; ++term) {  // the rounded value, then what it left
+        uint32_t b[kCount][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            b[e] = pack_bf16x2(v[e].x, v[e].y);
+        for (int k = 0; k < kCount; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[k][e] = pack_bf16x2(v[k][e].x, v[k][e].y);
+#pragma unroll
+        for (int k = 0; k < kCount; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
             if (term + 1 < kTerms)  // (a product with -1: packed operands have no sign modifier)
-              v[e] = __ffma2_rn(make_float2(bf16_lo(b[e]), bf16_hi(b[e])), make_float2(-1.f, -1.f), v[e]);
+              v[k][e] = __ffma2_rn(make_float2(bf16_lo(b[k][e]), bf16_hi(b[k][e])), make_float2(-1.f, -1.f), v[k][e]);
             else
-              chk = __fadd2_rn(chk, v[e]);  // the last remainders: NaN where x is not finite
-          }
-          sts128_op(sb + L::OFF_W + woff + term * 16384 + k * (kStride * 128), b[0], b[1], b[2], b[3]);
-        }
+              chk = __fadd2_rn(chk, v[k][e]);  // the last remainders: NaN where x is not finite
+#pragma unroll
+        for (int k = 0; k < kCount; ++k)
+          sts128_op(sb + L::OFF_W + woff + term * 16384 + k * (kStride * 128), b[k][0], b[k][1], b[k][2], b[k][3]);
       }
       if (!STATE_ONLY && !(chk.x + chk.y == chk.x + chk.y)) {
 #pragma unroll 1
@@ -498,74 +504,83 @@ __global__ void __launch_bounds__(kThreads, 1)
       signal(B_RDY_W, true);
     };
 
-    // ---- M of chunk c (quarters 2-3: rows i = row - 64, columns [16 cq, 16 cq + 16)) ----
-    const int mi = row - 64, r0 = 16 * cq;
-    const int md = min(max(mi - r0, -1), 16) + 1;  // row of the mask and skip tables
-    auto make_m = [&](auto below, int c, int st, uint32_t st_par) {
+    // ---- M of chunk c: rows i = row - 64 on quarters 2-3, in blocks of 16 columns.  Below the
+    //      diagonal a block costs about half of one on it.  With two heads a warp of quarter 2 takes
+    //      one block on the diagonal, a warp of quarter 3 one of each kind of one head; with one head
+    //      every block has its own warp (two are zero since the start) -----------------------
+    const int mi = row - 64;
+    const bool has_m = quarter >= 2 && (kHeads == 2 || quarter == 3 || cq < 2);
+    auto m_block = [&](auto below, int cb, int head, int st) {
       constexpr bool kBelow = decltype(below)::value;  // the block lies below the diagonal
-      const uint32_t par = static_cast<uint32_t>(c & 1);
-      if (!kBelow) wait(B_X + st, st_par);  // (the tables)
-      float r[kHeads];
-      uint32_t far = 0;
-#pragma unroll
-      for (int head = 0; head < kHeads; ++head) {
-        const float* tb = table(st, head);
-        r[head] = ex2_ftz(tb[G_GAM + mi] - tb[G_GAM + r0 + (kBelow ? 15 : 0)]);
-        if (!kBelow) far |= (steep[st * 2 + head] >> cq & 1u) << head;
-      }
-      if (c > 0) wait(B_PV, par ^ 1u);  // M is free
-      wait(B_G, par);
+      const int r0 = 16 * cb;
+      const float* tb = table(st, head);
+      const float r = ex2_ftz(tb[G_GAM + mi] - tb[G_GAM + r0 + (kBelow ? 15 : 0)]);
+      const bool far = !kBelow && (steep[st * 2 + head] >> cb & 1u);
       float v[16];
       tmem_ld16(tl + TM_G + r0, v);
       tmem_wait_ld();
       reg_fence(v);
+      uint32_t m[8];
+      if constexpr (kBelow) {
+        float u[16];
+        load16(tb + G_U + r0, u);
 #pragma unroll
-      for (int head = 0; head < kHeads; ++head) {
-        const float* tb = table(st, head);
-        uint32_t m[8];
-        if constexpr (kBelow) {
+        for (int k = 0; k < 8; ++k) {
+          const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
+                                      make_float2(r, r));
+          m[k] = pack_bf16x2(q.x, q.y);
+        }
+      } else {
+        const int md = min(max(mi - r0, -1), 16) + 1;  // row of the mask and skip tables
+        float skip[16];
+        load16(reinterpret_cast<const float*>(smem + L::OFF_SKIP + head * L::kSkipHead + md * L::kSkipPitch), skip);
+        float2 q[8];
+        if (!far) {
           float u[16];
-          load16(tb + G_U + r0, u);
+          load16(tb + G_V + r0, u);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            q[k] = __ffma2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
+                              make_float2(r, r), make_float2(skip[2 * k], skip[2 * k + 1]));
+        } else {
+          const float gi = tb[G_GAM + mi];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
-                                        make_float2(r[head], r[head]));
-            m[k] = pack_bf16x2(q.x, q.y);
-          }
-        } else {
-          float skip[16];
-          load16(reinterpret_cast<const float*>(smem + L::OFF_SKIP + head * L::kSkipHead + md * L::kSkipPitch), skip);
-          float2 q[8];
-          if (!(far >> head & 1u)) {
-            float u[16];
-            load16(tb + G_V + r0, u);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              q[k] = __ffma2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
-                                make_float2(r[head], r[head]), make_float2(skip[2 * k], skip[2 * k + 1]));
-          } else {
-            const float gi = tb[G_GAM + mi];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int j = r0 + 2 * k;
-              q[k].x = fmaf(v[2 * k], ex2_ftz(fminf(gi - tb[G_GAM + j], 0.f)) * tb[G_DT + j], skip[2 * k]);
-              q[k].y = fmaf(v[2 * k + 1], ex2_ftz(fminf(gi - tb[G_GAM + j + 1], 0.f)) * tb[G_DT + j + 1], skip[2 * k + 1]);
-            }
-          }
-          const uint4* mask = reinterpret_cast<const uint4*>(smem + L::OFF_MASK + md * L::kMaskPitch);
-#pragma unroll
-          for (int k4 = 0; k4 < 2; ++k4) {
-            const uint4 a = mask[k4];
-            m[4 * k4] = pack_bf16x2(q[4 * k4].x, q[4 * k4].y) & a.x;
-            m[4 * k4 + 1] = pack_bf16x2(q[4 * k4 + 1].x, q[4 * k4 + 1].y) & a.y;
-            m[4 * k4 + 2] = pack_bf16x2(q[4 * k4 + 2].x, q[4 * k4 + 2].y) & a.z;
-            m[4 * k4 + 3] = pack_bf16x2(q[4 * k4 + 3].x, q[4 * k4 + 3].y) & a.w;
+            const int j = r0 + 2 * k;
+            q[k].x = fmaf(v[2 * k], ex2_ftz(fminf(gi - tb[G_GAM + j], 0.f)) * tb[G_DT + j], skip[2 * k]);
+            q[k].y = fmaf(v[2 * k + 1], ex2_ftz(fminf(gi - tb[G_GAM + j + 1], 0.f)) * tb[G_DT + j + 1], skip[2 * k + 1]);
           }
         }
+        const uint4* mask = reinterpret_cast<const uint4*>(smem + L::OFF_MASK + md * L::kMaskPitch);
 #pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2)
-          sts128_op(sb + L::OFF_M + head * 8192 + sw128_off(mi, 2 * cq + c2), m[4 * c2], m[4 * c2 + 1], m[4 * c2 + 2],
-                    m[4 * c2 + 3]);
+        for (int k4 = 0; k4 < 2; ++k4) {
+          const uint4 a = mask[k4];
+          m[4 * k4] = pack_bf16x2(q[4 * k4].x, q[4 * k4].y) & a.x;
+          m[4 * k4 + 1] = pack_bf16x2(q[4 * k4 + 1].x, q[4 * k4 + 1].y) & a.y;
+          m[4 * k4 + 2] = pack_bf16x2(q[4 * k4 + 2].x, q[4 * k4 + 2].y) & a.z;
+          m[4 * k4 + 3] = pack_bf16x2(q[4 * k4 + 3].x, q[4 * k4 + 3].y) & a.w;
+        }
+      }
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2)
+        sts128_op(sb + L::OFF_M + head * 8192 + sw128_off(mi, 2 * cb + c2), m[4 * c2], m[4 * c2 + 1], m[4 * c2 + 2],
+                  m[4 * c2 + 3]);
+    };
+    auto make_m = [&](int c, int st, uint32_t st_par) {
+      wait(B_X + st, st_par);  // (the tables)
+      if (c > 0) wait2(B_PV, c - 1);  // M is free
+      wait(B_G, static_cast<uint32_t>(c & 1));
+      if (kHeads == 2) {
+        if (quarter == 2) {
+          m_block(std::false_type{}, cq & 1, cq >> 1, st);
+        } else {
+          m_block(std::false_type{}, 2 + (cq >> 1), cq & 1, st);
+          m_block(std::true_type{}, cq >> 1, cq & 1, st);
+        }
+      } else if (quarter == 3 && cq < 2) {
+        m_block(std::true_type{}, cq, 0, st);
+      } else {
+        m_block(std::false_type{}, cq, 0, st);
       }
       signal(B_RDY_M, true);
     };
@@ -579,18 +594,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ysm = (row >> 6) * 8192 + (16 * cq + (odd ? 8 : 0)) * 128 + 4 * ((row & 7) >> 1);
     const uint32_t ych = (row & 63) >> 3;
     auto outputs = [&](int c, int st) {
-      const uint32_t par = static_cast<uint32_t>(c & 1);
       float eg[16], qs[16], pv[16];
       load16(table(st, hh) + G_EG + 16 * cq, eg);
-      if (quarter < 2 || (quarter == 2 && cq >= 2) || c + 1 == n) wait(B_PV, par);  // (the others waited for it to write M)
-      wait(B_QS + (c & 1), static_cast<uint32_t>((c >> 1) & 1));
+      if (!has_m || c + 1 == n) wait2(B_PV, c);  // (the others waited for it to write M)
+      if (c + 1 == n) wait2(B_QS, c);  // (before that, the state's update waited for it)
       const bool bad = *any_bad != 0u;  // (written before this chunk's W was signalled)
-      tmem_ld16(tl + TM_PV + 16 * cq, pv);
+      tmem_ld16(tl + TM_PV + 64 * (c & 1) + 16 * cq, pv);
       tmem_ld16(tl + TM_QS + 64 * (c & 1) + 16 * cq, qs);
       tmem_wait_ld();
       reg_fence(pv);
       reg_fence(qs);
-      signal(B_RDY_D, false);
+      signal(B_RDY_D + (c & 1), false);
       float o[16];
 #pragma unroll
       for (int k = 0; k < 16; k += 2) {
@@ -636,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto update = [&](int c, int st) {
       const float dec = decs[st * 2 + hh];
       dprod *= dec;
-      if (c + 1 == n || (!STATE_ONLY && !w_all && !w_some))  // (the others waited for it to write W)
+      if (c + 1 == n || !has_w)  // (the others waited for it to write W)
         wait_ds(c);
       float v[kCols];
       if constexpr (kCols == 32)
@@ -651,7 +665,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         s[i] = r.x;
         s[i + 1] = r.y;
       }
-      if (!STATE_ONLY && c + 1 < n) publish_state(c + 1);
+      if (!STATE_ONLY && c + 1 < n) {
+        wait2(B_QS, c);  // the product that reads the last published state is done
+        publish_state();
+      }
     };
 
     // (buffer and stage of chunk c + 1, and their parity)
@@ -664,18 +681,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       if (c + 1 < n) {
-        using std::integral_constant;
-        if (STATE_ONLY) {
-          make_w(integral_constant<int, 32>{}, integral_constant<int, 2>{}, c + 1, st, st_par);
-        } else if (w_all) {
-          make_w(integral_constant<int, 16>{}, integral_constant<int, 3>{}, c + 1, st, st_par);
-        } else {
-          if (w_some) make_w(integral_constant<int, 8>{}, integral_constant<int, 2>{}, c + 1, st, st_par);
-          if (quarter == 3 && cq < 2)
-            make_m(std::true_type{}, c + 1, st, st_par);
-          else if (!w_some)
-            make_m(std::false_type{}, c + 1, st, st_par);
-        }
+        if (has_w)
+          make_w(c + 1, st, st_par);
+        else if (has_m)
+          make_m(c + 1, st, st_par);
+        else
+          wait(B_X + st, st_par);  // (the tables, for the outputs)
       }
       if (c >= 0) {
         update(c, prev);
@@ -740,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sdesc_sw128_f(bc + ks * 128, 16384, 1024), idesc_ds, part > 0 || ks > 0);
       commit_by(leader, &bars[B_DS + (STATE_ONLY ? c & 1 : 0)]);
     };
-    auto mma_pv = [&](int st) {
+    auto mma_pv = [&](int c, int st) {
       const uint32_t xo = L::OFF_ST + st * L::kStage;
 #pragma unroll
       for (int head = 0; head < kHeads; ++head)
@@ -755,15 +766,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             lbo = start + 8192 - L::OFF_Z0;
             start = L::OFF_Z0;
           }
-          mma_ss_by(leader, tm + TM_PV, sdesc_sw128_f(sb16 + start / 16, lbo, 1024), b, idesc_pv, head > 0 || ks > 0);
+          mma_ss_by(leader, tm + TM_PV + 64 * (c & 1), sdesc_sw128_f(sb16 + start / 16, lbo, 1024), b, idesc_pv, head > 0 || ks > 0);
         }
-      commit_by(leader, &bars[B_PV]);
+      commit_by(leader, &bars[B_PV + (c & 1)]);
     };
     auto mma_qs = [&](int c, int st) {
       const uint32_t bc = sb16 + kBc16 + st * kStage16;
 #pragma unroll
       for (int ks = 0; ks < NS / 16; ++ks)
-        mma_ts_by(leader, tm + TM_QS + 64 * (c & 1), tm + TM_SB + 64 * (c & 1) + 8 * ks,
+        mma_ts_by(leader, tm + TM_QS + 64 * (c & 1), tm + TM_SB + 8 * ks,
                   sdesc_sw128_f(bc + ((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) / 16, 16, 1024), idesc_qs, ks > 0);
       commit_by(leader, &bars[B_QS + (c & 1)]);
     };
@@ -782,19 +793,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_ds(c + 1, s1);
         commit_by(leader, &bars[B_EMPTY + s1]);
       } else {
-        if (c + 1 < n) {
-          if (!(ok = wait(B_RDY_M, next))) break;
-          if (c + 2 < n && !(ok = mma_g(s2, par2))) break;
-          if (!(ok = wait(B_RDY_W, next))) break;
-          if (!(ok = wait(B_RDY_S, next))) break;  // the update of chunk c has read W^T B
-          mma_ds(c + 1, s1);
-          mma_qs(c + 1, s1);
-        }
-        if (c >= 0 && !(ok = wait(B_RDY_D, next ^ 1u))) break;  // the outputs of chunk c have read their accumulators
-        if (c + 1 < n) {
-          mma_pv(s1);
-          commit_by(leader, &bars[B_EMPTY + s1]);
-        }
+        // the outputs of chunk c - 1 have read the buffers that chunk c + 1 takes
+        if (c >= 1 && !(ok = wait(B_RDY_D + static_cast<int>(next), static_cast<uint32_t>(((c - 1) >> 1) & 1)))) break;
+        if (c + 1 == n) break;
+        if (!(ok = wait(B_RDY_M, next))) break;
+        if (c + 2 < n && !(ok = mma_g(s2, par2))) break;
+        if (!(ok = wait(B_RDY_W, next))) break;
+        mma_pv(c + 1, s1);
+        if (!(ok = wait(B_RDY_S, next))) break;  // the update of chunk c has read W^T B
+        mma_ds(c + 1, s1);
+        mma_qs(c + 1, s1);
+        commit_by(leader, &bars[B_EMPTY + s1]);
       }
       s0 = s1;
       s1 = s2;
