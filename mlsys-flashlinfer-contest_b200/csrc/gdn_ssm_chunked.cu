@@ -63,8 +63,9 @@ using namespace sm100;
 
 constexpr int kComputeWarps = 16;
 constexpr int kComputeThreads = 32 * kComputeWarps;
-constexpr int kMmaWarp = 16, kGateWarp = 18;  // 17: TMA loads, 19: the second head's gates
+constexpr int kMmaWarp = 16, kLoadWarp = 17, kGateWarp = 18;  // and 19: the second head's gates
 constexpr int kThreads = kComputeThreads + 128;
+constexpr uint32_t kComputeBar = 1;  // named barrier of the compute warps
 constexpr uint64_t kTimeoutNs = 2000000000ull;  // 2 s per wait, then give up
 constexpr int kStages = 3;
 constexpr int kRows = 128;  // state rows of a CTA
@@ -121,7 +122,9 @@ enum : int {
   B_RDY_W = B_DONE + kStages, B_RDY_M,  // compute warps -> issue warp: operands of a chunk,
   B_RDY_S, B_RDY_D, B_RDY_D1,           // the state it starts from, its accumulators read
   // products done (two where a chunk's may complete before every warp has met the one before)
-  B_G, B_DS, B_DS1, B_PV, B_PV1, B_QS, B_QS1, B_END, kNumBars
+  B_G, B_DS, B_DS1, B_PV, B_PV1, B_QS, B_QS1, B_END,
+  B_STATE,  // the initial state landed
+  kNumBars
 };
 static_assert(kNumBars * 8 + 12 <= 256, "barrier area");
 
@@ -264,7 +267,7 @@ template <int P, int NS, bool STATE_ONLY>
 __global__ void __launch_bounds__(kThreads, 1)
     gdn_ssm_chunked_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_b,
                            const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ CUtensorMap tm_y,
-                           const Params p) {
+                           const __grid_constant__ CUtensorMap tm_s, const __grid_constant__ CUtensorMap tm_n, const Params p) {
   using L = Lay<P, NS>;
   constexpr int kHeads = L::kHeads, kKb = L::kKb;
   constexpr int kCols = NS / 4;  // state columns of a compute thread
@@ -313,7 +316,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
-  if (tid == 0) {
+  // ---- set-up.  The load thread makes the barriers and starts its loads at once. --------------
+  const uint32_t x_bytes = kHeads == 2 && !two ? 8192u : 16384u;
+  int bc_issued = 0, x_issued = 0;  // (load thread)
+  auto load_bc = [&](int c) {
+    const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
+    uint8_t* bc = smem + L::OFF_ST + st * L::kStage + L::kX;
+    mbar_arrive_expect_tx(&bars[B_BC + st], kKb * (STATE_ONLY ? 8192u : 16384u));
+#pragma unroll
+    for (int kb = 0; kb < kKb; ++kb) {
+      tma_load_3d(bc + kb * 16384, &tm_b, &bars[B_BC + st], 64 * kb, g, tok);
+      if (!STATE_ONLY) tma_load_3d(bc + kb * 16384 + 8192, &tm_c, &bars[B_BC + st], 64 * kb, g, tok);
+    }
+    bc_issued = c + 1;
+  };
+  auto load_x = [&](int c) {
+    const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
+    uint8_t* xs = smem + L::OFF_ST + st * L::kStage;
+    mbar_arrive_expect_tx(&bars[B_X + st], x_bytes);
+    tma_load_3d(xs, &tm_x, &bars[B_X + st], 0, h0, tok);
+    if (P == 128)
+      tma_load_3d(xs + 8192, &tm_x, &bars[B_X + st], 64, h0, tok);
+    else if (two)
+      tma_load_3d(xs + 8192, &tm_x, &bars[B_X + st], 0, h0 + 1, tok);
+    x_issued = c + 1;
+  };
+  // The initial and the final state pass through the space of W and M (64 KiB, free before the
+  // first chunk's and after the last one's) as boxes of 32 columns and 64 rows in the 128-byte
+  // swizzle: a thread's own row, read or written directly, is a transaction a lane.
+  const bool state_in = !STATE_ONLY && p.state != nullptr;
+  const int state_row = static_cast<int>((pc.seq * p.H + h0) * P);
+  if (warp == kLoadWarp && lane == 0) {
     for (int i = 0; i < kNumBars; ++i)
       mbar_init(&bars[i], i == B_RDY_W ? (STATE_ONLY ? kComputeWarps : kComputeWarps / 2) : i == B_RDY_M ? (kHeads == 2 ? 8 : 6)
                          : (i == B_RDY_S || i == B_RDY_D || i == B_RDY_D1 || (i >= B_DONE && i < B_DONE + kStages)) ? kComputeWarps
@@ -321,12 +354,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
     *abort_flag = 0u;
     *any_bad = 0u;
-    prefetch_tmap(&tm_x);
-    prefetch_tmap(&tm_b);
-    if (!STATE_ONLY) {
-      prefetch_tmap(&tm_c);
-      prefetch_tmap(&tm_y);
+    if (state_in) {
+      mbar_arrive_expect_tx(&bars[B_STATE], NS / 32 * (kHeads == 2 && !two ? 8192u : 16384u));
+#pragma unroll
+      for (int cb = 0; cb < NS / 32; ++cb) {
+        tma_load_2d(smem + L::OFF_W + cb * 16384, &tm_s, &bars[B_STATE], 32 * cb, state_row);
+        if (P == 128 || two) tma_load_2d(smem + L::OFF_W + cb * 16384 + 8192, &tm_s, &bars[B_STATE], 32 * cb, state_row + 64);
+      }
     }
+    for (int c = 0; c < min(n, kStages); ++c) {
+      load_bc(c);
+      load_x(c);
+    }
+    if (!STATE_ONLY) prefetch_tmap(&tm_y);
   }
   if (warp == 0) {
     tmem_alloc(tmem_slot, kTmemCols);
@@ -339,18 +379,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       sts128(sb + L::OFF_Z0 + 16 * i, 0u, 0u, 0u, 0u);
       sts128(sb + L::OFF_Z1 + 16 * i, 0u, 0u, 0u, 0u);
     }
-    for (int i = tid; i < 1024; i += kThreads) sts128(sb + L::OFF_M + 16 * i, 0u, 0u, 0u, 0u);
+    float skip[2] = {0.f, 0.f};
+    if (p.D) {
+      skip[0] = p.D[h0];
+      if (two) skip[1] = p.D[h0 + 1];
+    }
     for (int i = tid; i < 18 * 16; i += kThreads) {
       const int d = i / 16 - 1, j = i % 16;
       reinterpret_cast<uint16_t*>(smem + L::OFF_MASK + (d + 1) * L::kMaskPitch)[j] = j <= d ? 0xffffu : 0u;
       for (int head = 0; head < kHeads; ++head)
         reinterpret_cast<float*>(smem + L::OFF_SKIP + head * L::kSkipHead + (d + 1) * L::kSkipPitch)[j] =
-            j == d && p.D && (head == 0 || two) ? p.D[h0 + head] : 0.f;
+            j == d ? skip[head] : 0.f;
     }
   }
   if (kHeads == 2 && !two)  // the absent head's x
     for (int i = tid; i < kStages * 512; i += kThreads)
       sts128(sb + L::OFF_ST + (i >> 9) * L::kStage + 8192 + 16 * (i & 511), 0u, 0u, 0u, 0u);
+  // (gate warps: head gh, two tokens a lane)
+  const int gh = warp - kGateWarp;
+  const bool live = warp >= kGateWarp && (gh == 0 || (kHeads == 2 && two));
+  const unsigned short* pa = reinterpret_cast<const unsigned short*>(p.a) + h0 + (live ? gh : 0);
+  unsigned short raw[2] = {0, 0};
+  auto load_gates = [&](int c) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t t = bos + static_cast<int64_t>(c) * kChunk + 2 * lane + e;
+      if (live && t < pc.eos) raw[e] = pa[t * p.H];
+    }
+  };
+  float negA = 0.f, bias = 0.f;
+  if (live) {
+    negA = -expf(p.A_log[h0 + gh]) * kLog2e;
+    bias = p.dt_bias[h0 + gh];
+    load_gates(0);
+  }
   fence_async_smem();
   tc_fence_before();
   __syncthreads();
@@ -378,18 +440,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- initial state ------------------------------------------------------
     float s[kCols];
     float dprod = 1.f;  // decay of the piece
-    if (!STATE_ONLY && p.state && row_live) {
+    const uint32_t state_smem = sb + L::OFF_W + row * 128;
+    if (state_in) {
+      wait(B_STATE, 0);
 #pragma unroll
       for (int i = 0; i < kCols / 4; ++i) {
-        const float4 v = ld_stream_f4(p.state + row_off + 4 * i);
-        s[4 * i] = v.x;
-        s[4 * i + 1] = v.y;
-        s[4 * i + 2] = v.z;
-        s[4 * i + 3] = v.w;
+        const int col = kCols * cq + 4 * i;
+        const uint4 v = lds128(state_smem + (col >> 5) * 16384 + (((col >> 2 & 7) ^ (row & 7)) << 4));
+        s[4 * i] = __uint_as_float(v.x);
+        s[4 * i + 1] = __uint_as_float(v.y);
+        s[4 * i + 2] = __uint_as_float(v.z);
+        s[4 * i + 3] = __uint_as_float(v.w);
+      }
+      if (!row_live) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) s[i] = 0.f;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kCols; ++i) s[i] = 0.f;
+    }
+    if (!STATE_ONLY) {  // M's columns above the diagonal are zero from here on
+      if (state_in) named_sync(kComputeBar, kComputeThreads);  // (every thread has its state)
+      for (int i = tid; i < 1024; i += kComputeThreads) sts128(sb + L::OFF_M + 16 * i, 0u, 0u, 0u, 0u);
+      fence_async_smem();
+      named_sync(kComputeBar, kComputeThreads);
     }
     if (!STATE_ONLY) {
       for (int j = 0; j < pc.index; ++j) {  // through the pieces before this one
@@ -708,10 +783,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < kCols / 4; ++i)
           F[i * kComputeThreads] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
         if (cq == 0 && (row & 63) == 0) p.ws_dec[2 * u + (row >> 6)] = dprod;
-      } else if (last_piece && row_live) {
+      }
+    }
+    if (!STATE_ONLY && last_piece) {
+      // (this warp has met the last products that read W and M)
 #pragma unroll
-        for (int i = 0; i < kCols / 4; ++i)
-          st_stream_f4(p.new_state + row_off + 4 * i, make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]));
+      for (int i = 0; i < kCols / 4; ++i) {
+        const int col = kCols * cq + 4 * i;
+        sts128(state_smem + (col >> 5) * 16384 + (((col >> 2 & 7) ^ (row & 7)) << 4), __float_as_uint(s[4 * i]),
+               __float_as_uint(s[4 * i + 1]), __float_as_uint(s[4 * i + 2]), __float_as_uint(s[4 * i + 3]));
+      }
+      fence_async_smem();
+      if (!named_sync_or(kComputeBar, kComputeThreads, failed) && tid == 0) {
+#pragma unroll
+        for (int cb = 0; cb < NS / 32; ++cb) {
+          tma_store_2d(&tm_n, smem + L::OFF_W + cb * 16384, 32 * cb, state_row);
+          if (P == 128 || two) tma_store_2d(&tm_n, smem + L::OFF_W + cb * 16384 + 8192, 32 * cb, state_row + 64);
+        }
+        bulk_commit();
+        bulk_wait_all();
       }
     }
   } else if (warp == kMmaWarp) {
@@ -817,21 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     failed = !wait(B_END, 0) || !ok;
   } else if (warp >= kGateWarp) {
     // ======================= gate tables: warp 18 head 0, warp 19 head 1 =========
-    const int gh = warp - kGateWarp;
     if (gh < kHeads) {
-      const bool live = gh == 0 || two;
-      const float negA = live ? -expf(p.A_log[h0 + gh]) * kLog2e : 0.f;
-      const float bias = live ? p.dt_bias[h0 + gh] : 0.f;
-      const unsigned short* pa = reinterpret_cast<const unsigned short*>(p.a) + h0 + gh;
-      unsigned short raw[2] = {0, 0};  // two tokens a lane
-      auto load = [&](int c) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int64_t t = bos + static_cast<int64_t>(c) * kChunk + 2 * lane + e;
-          if (live && t < pc.eos) raw[e] = pa[t * p.H];
-        }
-      };
-      load(0);
       int buf = 0;
       uint32_t par = 0;
       for (int c = 0; c < n; ++c) {
@@ -848,7 +924,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           lg[e] = ok[e] ? fmaxf(lg[e], -256.f) : 0.f;
           dt[e] = ok[e] ? dt[e] : 0.f;
         }
-        if (c + 1 < n) load(c + 1);
+        if (c + 1 < n) load_gates(c + 1);
         const unsigned bad0 = __ballot_sync(0xffffffffu, !ok[0]), bad1 = __ballot_sync(0xffffffffu, !ok[1]);
         const int fb = min(bad0 ? 2 * (__ffs(bad0) - 1) : 64, bad1 ? 2 * (__ffs(bad1) - 1) + 1 : 64);
         const float pair = lg[0] + lg[1];
@@ -897,35 +973,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (lane == 0) {
     // ======================= TMA load and store thread =========================
-    const uint32_t x_bytes = kHeads == 2 && !two ? 8192u : 16384u;
     bool ok = true;
-    int bc_issued = 0, x_issued = 0;
-    auto load_bc = [&](int c) {
-      const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
-      uint8_t* bc = smem + L::OFF_ST + st * L::kStage + L::kX;
-      mbar_arrive_expect_tx(&bars[B_BC + st], kKb * (STATE_ONLY ? 8192u : 16384u));
-#pragma unroll
-      for (int kb = 0; kb < kKb; ++kb) {
-        tma_load_3d(bc + kb * 16384, &tm_b, &bars[B_BC + st], 64 * kb, g, tok);
-        if (!STATE_ONLY) tma_load_3d(bc + kb * 16384 + 8192, &tm_c, &bars[B_BC + st], 64 * kb, g, tok);
-      }
-      bc_issued = c + 1;
-    };
-    auto load_x = [&](int c) {
-      const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
-      uint8_t* xs = smem + L::OFF_ST + st * L::kStage;
-      mbar_arrive_expect_tx(&bars[B_X + st], x_bytes);
-      tma_load_3d(xs, &tm_x, &bars[B_X + st], 0, h0, tok);
-      if (P == 128)
-        tma_load_3d(xs + 8192, &tm_x, &bars[B_X + st], 64, h0, tok);
-      else if (two)
-        tma_load_3d(xs + 8192, &tm_x, &bars[B_X + st], 0, h0 + 1, tok);
-      x_issued = c + 1;
-    };
-    for (int c = 0; c < min(n, kStages); ++c) {
-      load_bc(c);
-      load_x(c);
-    }
     for (int c = 0; ok && c < n; ++c) {
       const int st = c % kStages;
       const uint32_t par = static_cast<uint32_t>((c / kStages) & 1);
@@ -982,8 +1030,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [T, heads, inner] bf16, box = 64 tokens x 1 head x 64 values, 128-byte swizzle; a small
-// cache per thread spares a caller that reuses its buffers the ~1 us of an encoding.
+// [T, heads, inner] bf16, box = 64 tokens x 1 head x 64 values, or (heads = 0) [T, inner] fp32,
+// box = 64 rows x 32 values; 128-byte swizzle.  A small cache per thread spares a caller that
+// reuses its buffers the ~1 us of an encoding.
 cudaError_t make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t heads, int64_t T) {
   struct Entry {
     const void* base;
@@ -1000,14 +1049,23 @@ cudaError_t make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t he
     }
   auto fn = encode_fn();
   if (!fn) return cudaErrorNotSupported;
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(T)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(inner) * 2, static_cast<cuuint64_t>(heads) * inner * 2};
-  cuuint32_t box[3] = {64, 1, 64};
-  cuuint32_t es[3] = {1, 1, 1};
-  if (fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
-         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return cudaErrorInvalidValue;
+  const cuuint64_t n = static_cast<cuuint64_t>(inner), h = static_cast<cuuint64_t>(heads), t = static_cast<cuuint64_t>(T);
+  const cuuint32_t es[3] = {1, 1, 1};
+  CUresult r;
+  if (heads) {
+    const cuuint64_t dims[3] = {n, h, t}, strides[2] = {n * 2, h * n * 2};
+    const cuuint32_t box[3] = {64, 1, 64};
+    r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    const cuuint64_t dims[2] = {n, t}, strides[1] = {n * 4};
+    const cuuint32_t box[2] = {32, 64};
+    r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, es,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
   cache[next] = Entry{base, inner, heads, T, *m};
   next = (next + 1) % kEntries;
   if (used < kEntries) ++used;
@@ -1063,18 +1121,21 @@ cudaError_t launch_one(const CUtensorMap* m, const Params& p, int64_t slots, cud
   if (e != cudaSuccess) return e;
   const int64_t ctas = slots * p.tiles;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-  kernel<<<static_cast<unsigned>(ctas), kThreads, bytes, s>>>(m[0], m[1], m[2], m[3], p);
+  kernel<<<static_cast<unsigned>(ctas), kThreads, bytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
   return cudaGetLastError();
 }
 
 template <int P, int NS>
 cudaError_t launch(const SsmArgs& a, const Cut& cut, void* ws, cudaStream_t s) {
-  CUtensorMap m[4];
+  CUtensorMap m[6];
+  memset(m, 0, sizeof(m));
   cudaError_t e;
   if ((e = make_map(&m[0], a.x, P, a.H, a.T)) != cudaSuccess) return e;
   if ((e = make_map(&m[1], a.B, NS, a.G, a.T)) != cudaSuccess) return e;
   if ((e = make_map(&m[2], a.C, NS, a.G, a.T)) != cudaSuccess) return e;
   if ((e = make_map(&m[3], a.out, P, a.H, a.T)) != cudaSuccess) return e;
+  if (a.state && (e = make_map(&m[4], a.state, NS, 0, a.N * a.H * P)) != cudaSuccess) return e;
+  if ((e = make_map(&m[5], a.new_state, NS, 0, a.N * a.H * P)) != cudaSuccess) return e;
   Params p{a.state, a.A_log, a.dt_bias, a.D, static_cast<const __nv_bfloat16*>(a.a), a.cu_seqlens,
            static_cast<__nv_bfloat16*>(a.out), a.new_state, static_cast<float*>(ws), nullptr, a.T, a.N, cut.seg,
            static_cast<int>(a.H), static_cast<int>(a.G), static_cast<int>(head_tiles(a.H, a.G, P))};
