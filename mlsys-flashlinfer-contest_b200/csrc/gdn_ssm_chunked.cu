@@ -207,6 +207,11 @@ __device__ __forceinline__ uint32_t elect_one() {
   return r;
 }
 
+// Programmatic dependent launch: lets the next launch start, and waits for the end of the one
+// before (at once when this launch was not made that way).
+__device__ __forceinline__ void dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The long form of a wait, out of line: polls with short naps, gives up after kTimeoutNs.
 __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait_nap(bar, parity, kTimeoutNs); }
 
@@ -311,8 +316,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h0 = g * group_heads + (tile % group_tiles) * kHeads;  // first head of the tile
   const bool two = kHeads == 2 && h0 + 1 < (g + 1) * group_heads;  // its second head exists
 
+  // The second launch may start once every CTA of the first has (it fills the SMs that the first
+  // leaves idle); a CTA waits for the first's end where it needs its results, and before it ends.
+  if (STATE_ONLY) dependency_launch();
   const Piece pc = find_piece<STATE_ONLY>(p, slot);
-  if (pc.seq < 0) return;
+  if (pc.seq < 0) {
+    if (!STATE_ONLY) dependency_wait();
+    return;
+  }
   const int64_t bos = pc.bos, Ltot = pc.eos - pc.bos;
   const bool last_piece = pc.index == pc.count - 1;
   const int n = static_cast<int>((Ltot + kChunk - 1) / kChunk);
@@ -332,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         st_stream_f4(p.new_state + row_off + 4 * i,
                      p.state ? ld_stream_f4(p.state + row_off + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f));
     }
+    if (!STATE_ONLY) dependency_wait();
     return;
   }
 
@@ -486,6 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       named_sync(kComputeBar, kComputeThreads);
     }
     if (!STATE_ONLY) {
+      if (pc.index > 0) dependency_wait();  // the first launch's results
       for (int j = 0; j < pc.index; ++j) {  // through the pieces before this one
         // (the slot among the pieces that are not a sequence's last)
         const int64_t u = (slot - pc.index - pc.seq + j) * p.tiles + tile;
@@ -1027,6 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     failed = !ok;
   }
   if (failed) atomicOr(&g_ssm_status, kStatusSsmTimeout);
+  if (!STATE_ONLY) dependency_wait();
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -1133,15 +1147,24 @@ Cut choose_cut(int64_t T, int64_t N, int64_t tiles, int sms) {
 }
 
 template <int P, int NS, bool STATE_ONLY>
-cudaError_t launch_one(const CUtensorMap* m, const Params& p, int64_t slots, cudaStream_t s) {
+cudaError_t launch_one(const CUtensorMap* m, const Params& p, int64_t slots, bool overlap, cudaStream_t s) {
   auto kernel = gdn_ssm_chunked_kernel<P, NS, STATE_ONLY>;
   constexpr int bytes = Lay<P, NS>::kBytes;
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
   const int64_t ctas = slots * p.tiles;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-  kernel<<<static_cast<unsigned>(ctas), kThreads, bytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], m[4], m[5], p);
 }
 
 template <int P, int NS>
@@ -1161,9 +1184,12 @@ cudaError_t launch(const SsmArgs& a, const Cut& cut, void* ws, cudaStream_t s) {
   if (cut.seg) {
     const int64_t inner = cut.slots - a.N;  // pieces that are not a sequence's last
     p.ws_dec = p.ws + inner * p.tiles * kRows * NS;
-    if (inner > 0 && (e = launch_one<P, NS, true>(m, p, inner, s)) != cudaSuccess) return e;
+    if (inner > 0) {
+      if ((e = launch_one<P, NS, true>(m, p, inner, false, s)) != cudaSuccess) return e;
+      return launch_one<P, NS, false>(m, p, cut.slots, true, s);
+    }
   }
-  return launch_one<P, NS, false>(m, p, cut.slots, s);
+  return launch_one<P, NS, false>(m, p, cut.slots, false, s);
 }
 
 }  // namespace

@@ -266,3 +266,38 @@ def test_one_long_sequence_among_many():
                                   torch.zeros(H, 64, 128))
         L.within(out[a:b], y, y_slack(ya, b - a))
         L.within(new[i], S, s_slack(Sa, b - a))
+
+
+def test_many_sequences_equal_one_call_each():
+    """More (sequence, tile) pairs than SMs: what runs beside a sequence changes no bit of it."""
+    from gdn_b200 import ssm
+    lens = [130, 0, 64, 700, 1, 65, 700, 320]
+    H = 64
+    m = make((sum(lens),), H, 64, 2, 128, seed=4)
+    st = torch.randn(len(lens), H, 64, 128, device="cuda")
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0)
+    out, new = ssm.run(m["x"], m["B"], m["C"], st, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)
+    for i, n in enumerate(lens):
+        a, b = int(cu[i]), int(cu[i + 1])
+        # (a short one alone takes the token-by-token kernel, a long one alone runs in pieces)
+        if n > 16 and ssm.workspace_bytes(n, 1, H, 2, 64, 128) == 0:
+            o, s = ssm.run(m["x"][a:b], m["B"][a:b], m["C"][a:b], st[i:i + 1], m["A_log"], m["a"][a:b], m["dt_bias"],
+                           m["D"], torch.tensor([0, n], device="cuda"))
+            assert torch.equal(out[a:b], o) and torch.equal(new[i:i + 1], s)
+    assert torch.equal(new[1], st[1])
+
+
+def test_one_long_sequence_among_some():
+    from gdn_b200 import ssm
+    lens = [40] * 20 + [4500] + [33] * 20
+    H = 8
+    assert ssm.workspace_bytes(sum(lens), len(lens), H, 1, 64, 128) > 0
+    m = make((sum(lens),), H, 64, 1, 128, seed=6)
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0)
+    out, new = ssm.run(m["x"], m["B"], m["C"], None, m["A_log"], m["a"], m["dt_bias"], m["D"], cu)
+    for i in (0, 19, 20, 21, 40):
+        a, b = int(cu[i]), int(cu[i + 1])
+        y, ya, S, Sa = L.scan_ref(*(m[k][a:b] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"],
+                                  torch.zeros(H, 64, 128))
+        L.within(out[a:b], y, y_slack(ya, b - a))
+        L.within(new[i], S, s_slack(Sa, b - a))
