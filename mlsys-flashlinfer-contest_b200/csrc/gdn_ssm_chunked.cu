@@ -30,15 +30,15 @@
 // the decays (e^gamma and the chunk's); tokens past the end are zeroed in x and B.
 //
 // Warp roles: warps 0-15 compute (four per TMEM lane quarter, each on a quarter of the
-// columns), warp 16 issues the MMAs, warp 17 the TMA loads, warps 18-19 compute the gate
-// tables of a head each.  The compute warps run, for chunk c: the operands W (quarters
-// 0-1, and pieces elsewhere) and M (quarters 2-3) of chunk c + 1, the state update of chunk c, the outputs of
-// chunk c.  Each step's matrix products were issued a step earlier, so no step waits for one
-// to run, and warps meet through mbarriers only (they may be in different steps).
-// What bounds the kernel is the compute warps' instructions, not HBM or the tensor pipe:
-// W ~60 a 16-byte piece of x (three terms), M ~45 a 32 x 16 block and head.  Outputs go from
-// registers to HBM: a warp's store covers two 64-byte row pieces, so nothing is gained by a tile
-// in shared memory, whose 16 KiB hold the third term of W instead.
+// columns), warp 16 issues the MMAs, warp 17 the TMA loads and stores, warps 18-19 compute the
+// gate tables of a head each.  The compute warps run, for chunk c: the operands W (quarters
+// 0-1) and M (quarters 2-3) of chunk c + 1, the state update of chunk c, the outputs of
+// chunk c, which go where the chunk's x was and leave by TMA.  Each step's products were issued a
+// step earlier, so no step waits for one to run, and warps meet through mbarriers only (they may
+// be in different steps).  What bounds the kernel is the compute warps' arithmetic and their
+// shared-memory accesses (issue slots ~50 % busy with 4.5 warps a scheduler), not HBM (29 %) or
+// the tensor pipe (30 %): 4 x 16384 tokens, 64 heads of 64, Ns 128: 670 us, 2.6 us a chunk;
+// with neither W nor M formed it would be 1.7 us.
 //
 // Few (sequence, head tile) pairs: sequences are cut into pieces of `seg` tokens.  A first
 // launch (STATE_ONLY) finds each piece's final state from zero and its decay; the second runs
@@ -141,6 +141,7 @@ struct Params {
   float* ws_dec;    // piece decays [slot][tile][2]
   int64_t T, N;
   int64_t seg;      // tokens of a piece (a multiple of 64); 0: sequences are whole
+  int64_t inner;    // pieces that are not a sequence's last, at most
   int H, G, tiles;  // tiles: head tiles of all groups
 };
 
@@ -500,8 +501,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!STATE_ONLY) {
       if (pc.index > 0) dependency_wait();  // the first launch's results
       for (int j = 0; j < pc.index; ++j) {  // through the pieces before this one
-        // (the slot among the pieces that are not a sequence's last)
-        const int64_t u = (slot - pc.index - pc.seq + j) * p.tiles + tile;
+        // (the slot among the pieces that are not a sequence's last; the bound holds for any cu_seqlens)
+        const int64_t u = min(slot - pc.index - pc.seq + j, p.inner - 1) * p.tiles + tile;
         const float dec = p.ws_dec[2 * u + hh];
         const float4* F = reinterpret_cast<const float4*>(p.ws) + u * (kRows * NS / 4) + tid;
 #pragma unroll
@@ -1179,13 +1180,12 @@ cudaError_t launch(const SsmArgs& a, const Cut& cut, void* ws, cudaStream_t s) {
   if (a.state && (e = make_map(&m[4], a.state, NS, 0, a.N * a.H * P)) != cudaSuccess) return e;
   if ((e = make_map(&m[5], a.new_state, NS, 0, a.N * a.H * P)) != cudaSuccess) return e;
   Params p{a.state, a.A_log, a.dt_bias, a.D, static_cast<const __nv_bfloat16*>(a.a), a.cu_seqlens,
-           static_cast<__nv_bfloat16*>(a.out), a.new_state, static_cast<float*>(ws), nullptr, a.T, a.N, cut.seg,
+           static_cast<__nv_bfloat16*>(a.out), a.new_state, static_cast<float*>(ws), nullptr, a.T, a.N, cut.seg, cut.slots - a.N,
            static_cast<int>(a.H), static_cast<int>(a.G), static_cast<int>(head_tiles(a.H, a.G, P))};
   if (cut.seg) {
-    const int64_t inner = cut.slots - a.N;  // pieces that are not a sequence's last
-    p.ws_dec = p.ws + inner * p.tiles * kRows * NS;
-    if (inner > 0) {
-      if ((e = launch_one<P, NS, true>(m, p, inner, false, s)) != cudaSuccess) return e;
+    p.ws_dec = p.ws + p.inner * p.tiles * kRows * NS;
+    if (p.inner > 0) {
+      if ((e = launch_one<P, NS, true>(m, p, p.inner, false, s)) != cudaSuccess) return e;
       return launch_one<P, NS, false>(m, p, cut.slots, true, s);
     }
   }
