@@ -10,6 +10,7 @@
 // of a call from ~30 us (Python checks + ctypes) to a few microseconds, which is
 // most of the latency of a small decode or prefill call.
 #include <torch/extension.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -350,6 +351,12 @@ void expect(const at::Tensor& ref, const at::Tensor& t, const char* name, at::Sc
   TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape_text(shape), ", got ", shape_text(t.sizes()));
 }
 
+// An output on x's device, straight from the allocator: the dispatcher is a third of the cost of
+// a small at::empty, and a token's call makes up to three of them.
+at::Tensor make_empty(const at::Tensor& x, at::IntArrayRef shape, at::ScalarType s) {
+  return at::detail::empty_cuda(shape, s, x.device(), c10::nullopt);
+}
+
 int dtype16(const at::Tensor& x) {
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
                    "x must be bfloat16 or float16");
@@ -386,7 +393,7 @@ std::vector<at::Tensor> conv_outputs(const at::Tensor& x, std::vector<int64_t>& 
       expect(x, (*given)[i], "outputs", x.scalar_type(), shape);
       outs.push_back((*given)[i]);
     } else {
-      outs.push_back(at::empty(shape, x.options()));
+      outs.push_back(make_empty(x, shape, x.scalar_type()));
     }
     ptrs.push_back(outs.back().data_ptr());
   }
@@ -423,7 +430,7 @@ std::tuple<std::vector<at::Tensor>, at::Tensor> conv(
   if (new_state.has_value())
     expect(x, *new_state, "new_state", x.scalar_type(), {N, W - 1, D});
   else
-    new_state = at::empty({N, W - 1, D}, x.options());
+    new_state = make_empty(x, {N, W - 1, D}, x.scalar_type());
   std::vector<void*> ptrs;
   std::vector<at::Tensor> outs = conv_outputs(x, splits, outputs, ptrs);
   const c10::cuda::CUDAGuard guard(x.device());
@@ -509,15 +516,15 @@ std::tuple<at::Tensor, at::Tensor> ssm(const at::Tensor& x, const at::Tensor& B,
   if (output.has_value())
     expect(x, *output, "output", at::kBFloat16, x.sizes());
   else
-    output = at::empty(x.sizes(), x.options());
+    output = make_empty(x, x.sizes(), x.scalar_type());
   if (new_state.has_value())
     expect(x, *new_state, "new_state", at::kFloat, ss);
   else
-    new_state = at::empty(ss, x.options().dtype(at::kFloat));
+    new_state = make_empty(x, ss, at::kFloat);
   const c10::cuda::CUDAGuard guard(x.device());
   const size_t ws_bytes = gdn_ssm_workspace_bytes(T, N, z.H, z.G, z.P, z.Ns);
   at::Tensor ws;
-  if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
+  if (ws_bytes) ws = make_empty(x, {static_cast<int64_t>(ws_bytes)}, at::kByte);
   check_rc(gdn_ssm(x.data_ptr(), B.data_ptr(), C.data_ptr(), state_ptr(state), A_log.data_ptr<float>(),
                    a.data_ptr(), dt_bias.data_ptr<float>(), state_ptr(D), cu_seqlens.data_ptr<int64_t>(),
                    output->data_ptr(), new_state->data_ptr<float>(), T, N, z.H, z.G, z.P, z.Ns,
@@ -544,7 +551,7 @@ at::Tensor ssm_pool(const at::Tensor& x, const at::Tensor& B, const at::Tensor& 
   if (output.has_value())
     expect(x, *output, "output", at::kBFloat16, x.sizes());
   else
-    output = at::empty(x.sizes(), x.options());
+    output = make_empty(x, x.sizes(), x.scalar_type());
   const c10::cuda::CUDAGuard guard(x.device());
   check_rc(gdn_ssm_pool(x.data_ptr(), B.data_ptr(), C.data_ptr(), A_log.data_ptr<float>(), a.data_ptr(),
                         dt_bias.data_ptr<float>(), state_ptr(D), state_pool.data_ptr(),
@@ -590,7 +597,7 @@ std::vector<at::Tensor> rms_norm(const at::Tensor& x, const at::Tensor& weight, 
   if (output.has_value())
     expect(x, *output, "output", ot, x.sizes());
   else
-    output = at::empty(x.sizes(), x.options().dtype(ot));
+    output = make_empty(x, x.sizes(), ot);
   ret.push_back(*output);
   if (fp8) {
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -598,14 +605,14 @@ std::vector<at::Tensor> rms_norm(const at::Tensor& x, const at::Tensor& weight, 
       shape.back() = D / group;
     else
       shape.pop_back();
-    ret.push_back(at::empty(shape, x.options().dtype(at::kFloat)));
+    ret.push_back(make_empty(x, shape, at::kFloat));
   }
   float* scale = fp8 ? ret.back().data_ptr<float>() : nullptr;
   if (residual.has_value()) {
     if (residual_out.has_value())
       expect(x, *residual_out, "residual_out", x.scalar_type(), x.sizes());
     else
-      residual_out = at::empty(x.sizes(), x.options());
+      residual_out = make_empty(x, x.sizes(), x.scalar_type());
     ret.push_back(*residual_out);
   }
   const c10::cuda::CUDAGuard guard(x.device());
