@@ -319,6 +319,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) gdn_conv_kernel(ConvPa
 
 // T tokens of one sequence per (block row, thread): the state rows and the first
 // tokens are all loaded before any is used, and a thread writes only what it read.
+// Four channels a thread: 256 x 4 tokens x 8192 channels in 14.5 us (eight: 15.9; one token ahead
+// instead of four: 18.6), of which ~2 are the launch; the floor is 9.
 template <class T, int W, bool SILU, int kCh>
 __global__ void __launch_bounds__(kThreads) gdn_conv_pool_kernel(ConvParams p) {
   using R = Raw<kCh>;
