@@ -461,10 +461,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[b]);
     };
-    // After a timeout a thread waits for nothing any more (its results are garbage, the status
-    // word says so) and leaves the loop.
+    // After a timeout a lane waits for nothing any more (its results are garbage, the status word
+    // says so), and its warp leaves the loop.  A test may answer the lanes differently, and the
+    // tensor-memory instructions behind it are the whole warp's: they meet first.  (2 % of the
+    // kernel's time; votes on the test instead were 3 %.)
     auto wait = [&](int b, uint32_t parity) {
       if (!failed && !mbar_test(&bars[b], parity)) failed = !wait_long(&bars[b], parity);
+      __syncwarp();
       tc_fence_after();
     };
     auto table = [&](int buf, int head) { return gates + (buf * 2 + head) * kGateFloats; };
@@ -783,8 +786,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int st = 0, prev = 0;
     uint32_t st_par = 0;
     for (int c = -1; c < n; ++c) {
-      if (failed) *abort_flag = 1u;
-      if (*abort_flag) {
+      if (__any_sync(0xffffffffu, failed || *abort_flag != 0u)) {
+        *abort_flag = 1u;
         failed = true;
         break;
       }
@@ -979,8 +982,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float top = __shfl_sync(0xffffffffu, gt[1], lane | 7);
         const float g63 = __shfl_sync(0xffffffffu, gt[1], 31);
         const unsigned far = __ballot_sync(0xffffffffu, first - top > 64.f);
-        if (c >= kStages && !failed && !mbar_test(&bars[B_DONE + buf], par ^ 1u))
-          failed = !wait_long(&bars[B_DONE + buf], par ^ 1u);
+        if (c >= kStages && !__all_sync(0xffffffffu, mbar_test(&bars[B_DONE + buf], par ^ 1u)))
+          failed = !__all_sync(0xffffffffu, wait_long(&bars[B_DONE + buf], par ^ 1u));
         if (failed) break;
         float* tb = gates + (buf * 2 + gh) * kGateFloats;
         *reinterpret_cast<float2*>(tb + G_GAM + 2 * lane) = make_float2(gt[0], gt[1]);
@@ -1041,8 +1044,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     failed = !ok;
   }
   if (failed) atomicOr(&g_ssm_status, kStatusSsmTimeout);
-  if (!STATE_ONLY) dependency_wait();
   __syncwarp();
+  if (!STATE_ONLY) dependency_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
