@@ -219,71 +219,98 @@ __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) { return 
 struct Piece {
   int64_t seq, bos, eos;  // sequence (-1: none) and the piece's tokens
   int index, count;       // of the sequence's pieces
+  int before;             // inner pieces of the sequences before this one (where index > 0)
 };
 
-// The piece of slot `slot`: sequences in order, each with max(1, ceil(length / seg)) pieces,
-// less its last one with STATE_ONLY.  Every warp finds it by itself, 128 sequences at a time (four
-// consecutive ones a lane, all loads at once: the loads' latency and 64-bit divisions, 32
-// sequences at a time, were 1.7 us of a short call's CTA).
+// The pieces of a sequence number max(1, ceil(length / seg)); all but its last are inner pieces,
+// numbered through the sequences in order.  Four consecutive sequences of a lane, from n0 on: their
+// inner pieces `cnt`, bounds and the sum over this lane and those before it.
+struct Inner {
+  int b[4], e[4], cnt[4], sum, incl;
+};
+__device__ __forceinline__ Inner inner_pieces(const Params& p, int64_t n0) {
+  const int lane = threadIdx.x & 31;
+  const unsigned seg = static_cast<unsigned>(p.seg);
+  Inner r;
+  int64_t c[5];
+#pragma unroll
+  for (int u = 0; u < 5; ++u) c[u] = p.cu[min(n0 + u, p.N)];
+  r.sum = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    r.b[u] = static_cast<int>(min(max(c[u], int64_t(0)), p.T));
+    r.e[u] = static_cast<int>(min(max(c[u + 1], static_cast<int64_t>(r.b[u])), p.T));
+    const unsigned len = static_cast<unsigned>(r.e[u] - r.b[u]);
+    r.cnt[u] = n0 + u < p.N && len > seg ? static_cast<int>((len + seg - 1) / seg) - 1 : 0;
+    r.sum += r.cnt[u];
+  }
+  r.incl = r.sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, r.incl, d);
+    if (lane >= d) r.incl += y;
+  }
+  return r;
+}
+
+// The piece of slot `slot`: inner pieces first (the longest run first), then the sequences' last
+// ones, whose sequence is the slot itself.  A warp finds an inner piece by itself, 128 sequences
+// at a time, and so what lies before a last piece that is not the only one; were all pieces in the
+// sequences' order, every CTA would search: 4096 sequences of 64 tokens took 4.6 ms instead of 1.7.
 template <bool STATE_ONLY>
 __device__ __forceinline__ Piece find_piece(const Params& p, int64_t slot) {
   const int lane = threadIdx.x & 31;
-  Piece r{-1, 0, 0, 0, 1};
-  if (p.seg == 0) {
-    if (slot >= p.N) return r;
-    r.seq = slot;
-    r.bos = min(max(p.cu[slot], int64_t(0)), p.T);
-    r.eos = min(max(p.cu[slot + 1], r.bos), p.T);
+  Piece r{-1, 0, 0, 0, 1, 0};
+  if (p.seg == 0 || (!STATE_ONLY && slot >= p.inner)) {
+    const int64_t seq = p.seg == 0 ? slot : slot - p.inner;
+    if (seq >= p.N) return r;
+    r.seq = seq;
+    r.bos = min(max(p.cu[seq], int64_t(0)), p.T);
+    r.eos = min(max(p.cu[seq + 1], r.bos), p.T);
+    if (p.seg == 0 || r.eos - r.bos <= p.seg) return r;
+    r.count = static_cast<int>((r.eos - r.bos + p.seg - 1) / p.seg);
+    r.index = r.count - 1;
+    r.bos += r.index * p.seg;
+    for (int64_t base = 0; base < seq; base += 128) {
+      const int64_t n0 = base + 4 * lane;
+      const Inner in = inner_pieces(p, n0);
+      int sum = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sum += n0 + u < seq ? in.cnt[u] : 0;
+      r.before += __reduce_add_sync(0xffffffffu, sum);
+    }
     return r;
   }
-  const unsigned seg = static_cast<unsigned>(p.seg);
   int left = static_cast<int>(slot);  // (slots are fewer than 2^31)
   for (int64_t base = 0; base < p.N; base += 128) {
-    const int64_t n0 = base + 4 * lane;
-    int64_t c[5];
-#pragma unroll
-    for (int u = 0; u < 5; ++u) c[u] = p.cu[min(n0 + u, p.N)];
-    int b[4], e[4], cnt[4], sum = 0;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      b[u] = static_cast<int>(min(max(c[u], int64_t(0)), p.T));
-      e[u] = static_cast<int>(min(max(c[u + 1], static_cast<int64_t>(b[u])), p.T));
-      const unsigned len = static_cast<unsigned>(e[u] - b[u]);
-      cnt[u] = n0 + u < p.N ? static_cast<int>(len > seg ? (len + seg - 1) / seg : 1u) - (STATE_ONLY ? 1 : 0) : 0;
-      sum += cnt[u];
-    }
-    int incl = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += y;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, left < incl);
+    const Inner in = inner_pieces(p, base + 4 * lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, left < in.incl);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      int at = left - (incl - sum), k = 0;  // (lane src: the slot among its four sequences' pieces)
+      int at = left - (in.incl - in.sum), k = 0;  // (lane src: the slot among its four sequences' pieces)
 #pragma unroll
       for (int u = 0; u < 3; ++u)
-        if (k == u && at >= cnt[u]) {
-          at -= cnt[u];
+        if (k == u && at >= in.cnt[u]) {
+          at -= in.cnt[u];
           k = u + 1;
         }
-      int bb = b[0], ee = e[0], cc = cnt[0];
+      int bb = in.b[0], ee = in.e[0], cc = in.cnt[0];
 #pragma unroll
       for (int u = 1; u < 4; ++u)
         if (k == u) {
-          bb = b[u];
-          ee = e[u];
-          cc = cnt[u];
+          bb = in.b[u];
+          ee = in.e[u];
+          cc = in.cnt[u];
         }
       r.seq = base + 4 * src + __shfl_sync(0xffffffffu, k, src);
       r.index = __shfl_sync(0xffffffffu, at, src);
-      r.count = __shfl_sync(0xffffffffu, cc, src) + (STATE_ONLY ? 1 : 0);
+      r.count = __shfl_sync(0xffffffffu, cc, src) + 1;
+      r.before = static_cast<int>(slot) - r.index;
       r.bos = __shfl_sync(0xffffffffu, bb, src) + r.index * p.seg;
       r.eos = min(r.bos + p.seg, static_cast<int64_t>(__shfl_sync(0xffffffffu, ee, src)));
       return r;
     }
-    left -= __shfl_sync(0xffffffffu, incl, 31);
+    left -= __shfl_sync(0xffffffffu, in.incl, 31);
   }
   return r;
 }
@@ -318,11 +345,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool two = kHeads == 2 && h0 + 1 < (g + 1) * group_heads;  // its second head exists
 
   // The second launch may start once every CTA of the first has (it fills the SMs that the first
-  // leaves idle); a CTA waits for the first's end where it needs its results, and before it ends.
+  // leaves idle).  Its CTAs wait for the first's end where they need its results, and one before it
+  // ends, so that the second does not end first.  (Were that all of them, the first's time would
+  // not overlap more than a CTA an SM: 1024 sequences of 32 tokens and one of 32 thousand, 64 heads,
+  // 2247 instead of 2572 us.)
   if (STATE_ONLY) dependency_launch();
+  const bool ends_last = !STATE_ONLY && blockIdx.x == 0;
   const Piece pc = find_piece<STATE_ONLY>(p, slot);
   if (pc.seq < 0) {
-    if (!STATE_ONLY) dependency_wait();
+    if (ends_last) dependency_wait();
     return;
   }
   const int64_t bos = pc.bos, Ltot = pc.eos - pc.bos;
@@ -344,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         st_stream_f4(p.new_state + row_off + 4 * i,
                      p.state ? ld_stream_f4(p.state + row_off + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f));
     }
-    if (!STATE_ONLY) dependency_wait();
+    if (ends_last) dependency_wait();
     return;
   }
 
@@ -504,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!STATE_ONLY) {
       if (pc.index > 0) dependency_wait();  // the first launch's results
       for (int j = 0; j < pc.index; ++j) {  // through the pieces before this one
-        // (the slot among the pieces that are not a sequence's last; the bound holds for any cu_seqlens)
-        const int64_t u = min(slot - pc.index - pc.seq + j, p.inner - 1) * p.tiles + tile;
+        // (the bound holds for any cu_seqlens)
+        const int64_t u = min(static_cast<int64_t>(pc.before) + j, p.inner - 1) * p.tiles + tile;
         const float dec = p.ws_dec[2 * u + hh];
         const float4* F = reinterpret_cast<const float4*>(p.ws) + u * (kRows * NS / 4) + tid;
 #pragma unroll
@@ -1045,7 +1076,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (failed) atomicOr(&g_ssm_status, kStatusSsmTimeout);
   __syncwarp();
-  if (!STATE_ONLY) dependency_wait();
+  if (ends_last) dependency_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {

@@ -301,3 +301,24 @@ def test_one_long_sequence_among_some():
                                   torch.zeros(H, 64, 128))
         L.within(out[a:b], y, y_slack(ya, b - a))
         L.within(new[i], S, s_slack(Sa, b - a))
+
+
+def test_long_sequences_among_hundreds():
+    """More sequences than one round of the search for a piece covers (128), with several cut ones."""
+    from gdn_b200 import ssm
+    lens = [20 + i % 50 for i in range(400)]
+    lens[3], lens[140], lens[399], lens[200] = 4000, 5001, 2500, 0
+    H = 8
+    assert ssm.workspace_bytes(sum(lens), len(lens), H, 1, 64, 128) > 0
+    m = make((sum(lens) + 70,), H, 64, 1, 128, seed=7)
+    st = torch.randn(len(lens), H, 64, 128, device="cuda")
+    cu = torch.tensor([6] + lens, device="cuda").cumsum(0)
+    out = torch.full_like(m["x"], 7.0)
+    _, new = ssm.run(m["x"], m["B"], m["C"], st, m["A_log"], m["a"], m["dt_bias"], m["D"], cu, output=out)
+    assert (out[:6] == 7).all() and (out[int(cu[-1]):] == 7).all()
+    assert torch.equal(new[200], st[200])
+    for i in (0, 2, 3, 4, 127, 128, 139, 140, 141, 199, 201, 255, 256, 398, 399):
+        a, b = int(cu[i]), int(cu[i + 1])
+        y, ya, S, Sa = L.scan_ref(*(m[k][a:b] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"], st[i])
+        L.within(out[a:b], y, y_slack(ya, b - a))
+        L.within(new[i], S, s_slack(Sa, b - a))
