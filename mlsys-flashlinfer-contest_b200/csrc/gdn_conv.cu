@@ -131,14 +131,15 @@ __device__ __forceinline__ void load_weights(const ConvParams& p, int64_t c0, fl
 }
 
 // silu of two values with one reciprocal: 1 / (a b) gives both, a = 1 + 2^(-x log2 e).  The
-// exponents are held below 2^60, so that the product stays finite (below x = -41.6 the result is
-// x 2^-60 instead of its even smaller value); fminf also keeps a NaN to its own result.  MUFU
+// exponents are held below 2^60, so that the product stays finite; where one would exceed that,
+// x < -41.5, the sigmoid is 0 instead of less than 2^-59 (x 2^-60 would be 1e20 for the type's
+// lowest value); -inf gives NaN, as in the formula.  fminf also keeps a NaN to its own result.  MUFU
 // operations bound the convolution next to HBM: three for two values instead of four.
 __device__ __forceinline__ void silu2(float& x, float& y) {
   const float a = 1.0f + ex2_ftz(fminf(-x * kLog2e, 60.f)), b = 1.0f + ex2_ftz(fminf(-y * kLog2e, 60.f));
   const float r = rcp_approx(a * b);
-  x *= r * b;
-  y *= r * a;
+  x *= x < -41.5f ? 0.f : r * b;
+  y *= y < -41.5f ? 0.f : r * a;
 }
 
 // One output row from the window (W - 1 earlier rows, oldest first) and the current row.

@@ -187,3 +187,27 @@ def test_refusals():
     new = torch.zeros(1, 3, 64, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError, match="overlaps"):
         conv.run(*ok[:3], new, m["cu"], new_state=new)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("pool", [False, True])
+def test_lowest_values(pool, dtype):
+    """silu of sums at the bottom of the range is 0, of -inf NaN, and the neighbouring channels see neither."""
+    from gdn_b200 import conv
+    m = make([40], 64, 4, dtype, True, True, seed=9)
+    m["x"][3, ::2] = torch.finfo(dtype).min
+    m["x"][20, 1] = -1e4
+    m["x"][30, 2::2] = -float("inf")
+    w = m["weight"].abs().clamp(0.1, 1.0)
+    if pool:
+        pl = m["state"].clone()
+        out = conv.run_pool(m["x"][None], w, m["bias"], pl, torch.zeros(1, dtype=torch.int32, device="cuda"))[0]
+    else:
+        out, _ = conv.run(m["x"], w, m["bias"], m["state"], m["cu"])
+    ref, mag, _ = L.conv_ref(m["x"].clamp(min=torch.finfo(dtype).min), w, m["bias"], m["state"][0])
+    inf = torch.zeros(40, 64, dtype=torch.bool)
+    inf[30:34, 2::2] = True
+    low = (mag > 1e3) & ~inf
+    got = L.d(out)
+    assert low[3:7, ::2].all() and (got[low] == 0).all() and got[inf].isnan().all()
+    L.within(out[~(low | inf).to(out.device)], ref[~(low | inf)], SLACK * mag[~(low | inf)])
