@@ -321,8 +321,9 @@ enum gdn_dtype { GDN_BF16 = 0, GDN_F16 = 1 };
  * All tensors are of `dtype`; width is 2, 3 or 4; dim and x_row_stride are multiples
  * of 8 and every buffer 16-byte aligned.  Sums are fp32, rounded once.  A sequence of
  * length 0 keeps its state.  Rows of no sequence (before cu_seqlens[0] or from
- * cu_seqlens[N] on) are left as they were.  new_state may not overlap state, and the
- * outputs nothing else.  cu_seqlens is read only on the device, clamped to [0, T].
+ * cu_seqlens[N] on) are left as they were.  new_state and the outputs may not overlap
+ * x (from its first row to its last), state, weight, bias or one another.  silu is
+ * -0 for sums below -41.5, NaN for -inf.  cu_seqlens is read only on the device, clamped to [0, T].
  */
 int gdn_conv(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
              const void *state, const int64_t *cu_seqlens, void *const *outputs,
@@ -335,7 +336,7 @@ int gdn_conv(const void *x, int64_t x_row_stride, const void *weight, const void
  *   x         [B, seq_len, dim], token t of sequence i at
  *             x + i * x_batch_stride + t * x_row_stride elements
  *   state_pool [pool_size, width - 1, dim]; in_slots, out_slots as in gdn_decode_pool
- *   outputs   [B, seq_len, widths[i]], contiguous
+ *   outputs   [B, seq_len, widths[i]], contiguous, overlapping nothing
  * Slots as for gdn_decode_pool: a negative or out-of-range read slot means a zero
  * state, such a write slot no write; two sequences writing the same slot, or one
  * reading a slot another writes, race.
@@ -354,7 +355,8 @@ int gdn_conv_pool(const void *x, int64_t x_batch_stride, int64_t x_row_stride, c
  *   state     [N, H, P, Ns] fp32 or NULL   a        [T, H] bf16
  *   A_log, dt_bias [H] fp32                D        [H] fp32 or NULL (no skip term)
  *   cu_seqlens [N+1] int64, device         output   [T, H, P] bf16
- *   new_state [N, H, P, Ns] fp32, may not overlap state
+ *   new_state [N, H, P, Ns] fp32
+ * output and new_state may not overlap an input or one another.
  * P (head_dim) and Ns (state_dim) are 64 or 128; num_heads is a multiple of num_groups.
  * The state is in the k-last layout of gdn_prefill.  A sequence of length 0 keeps its
  * state.  Rows of no sequence are left as they were.  Buffers need 16-byte alignment.
@@ -375,6 +377,7 @@ size_t gdn_ssm_workspace_bytes(int64_t total_seq_len, int64_t num_seqs, int64_t 
  * GDN_POOL_NO_STATE_UPDATE:
  *   x [B, seq_len, H, P], B, C [B, seq_len, G, Ns], a [B, seq_len, H], output as x
  *   state_pool [pool_size, H, P, Ns]; slots as in gdn_decode_pool
+ * output may not overlap another tensor.
  */
 int gdn_ssm_pool(const void *x, const void *B, const void *C, const float *A_log, const void *a,
                  const float *dt_bias, const float *D, void *state_pool, int state_dtype,
@@ -397,6 +400,8 @@ int gdn_ssm_pool(const void *x, const void *B, const void *C, const float *A_log
  *   output    [rows, dim] of `dtype`, or with `scale` e4m3 (1 byte): y / scale with
  *   scale     [rows] (group_size 0) or [rows, dim / 128] (group_size 128) fp32:
  *             max |y| of the row or group / 448 (1 where that maximum is below 2^-100)
+ * A 16-bit output or residual_out may be one of the inputs that is contiguous, as a whole;
+ * no other overlap is allowed.  Squares are summed in fp32: above 1e18 they overflow.
  * y is fp32 up to the output's one rounding.  dim is a multiple of 8 (of 128 with
  * group_size 128) up to 16384; strides are multiples of 8, buffers 16-byte aligned.
  */

@@ -415,6 +415,33 @@ static bool overlap(const void* p, size_t np, const void* q, size_t nq) {
   return a < b + nq && b < a + np;
 }
 
+struct Range {
+  const void* p;
+  size_t bytes;
+};
+// One of the ranges that are written shares a byte with another of them or with one that is read.
+static bool any_overlap(const Range* written, int nw, const Range* read, int nr) {
+  for (int i = 0; i < nw; ++i) {
+    for (int j = i + 1; j < nw; ++j)
+      if (overlap(written[i].p, written[i].bytes, written[j].p, written[j].bytes)) return true;
+    for (int j = 0; j < nr; ++j)
+      if (overlap(written[i].p, written[i].bytes, read[j].p, read[j].bytes)) return true;
+  }
+  return false;
+}
+
+// The outputs of a convolution of `rows` rows, and `extra` that it writes too, against what it reads
+// (x spans x_elems elements; the neighbours' rows are read while a row is written).
+static bool conv_overlap(const gdn::ConvArgs& a, int64_t rows, int64_t x_elems, Range extra, const void* state) {
+  Range w[gdn::kMaxConvOutputs + 1];
+  for (int i = 0; i < a.out.count; ++i) w[i] = {a.out.ptr[i], static_cast<size_t>(rows) * a.out.width[i] * 2};
+  w[a.out.count] = extra;
+  const size_t wide = static_cast<size_t>(a.D) * 2;
+  const Range r[4] = {{a.x, rows ? static_cast<size_t>(x_elems) * 2 : 0}, {a.weight, wide * a.W}, {a.bias, wide},
+                      {state, extra.bytes}};
+  return any_overlap(w, a.out.count + 1, r, 4);
+}
+
 static int check_conv(const void* x, int64_t x_batch, int64_t x_row, const void* weight, const void* bias,
                       void* const* outputs, const int64_t* widths, int count, int64_t T, int64_t N,
                       int64_t D, int64_t W, int dtype, int flags, gdn::ConvArgs* a) {
@@ -471,6 +498,8 @@ int gdn_conv(const void* x, int64_t x_row_stride, const void* weight, const void
     return fail(GDN_ERR_VALUE, "state and new_state must be 16-byte and cu_seqlens 8-byte aligned");
   const size_t bytes = static_cast<size_t>(N) * (W - 1) * D * 2;
   if (overlap(state, bytes, new_state, bytes)) return fail(GDN_ERR_VALUE, "new_state overlaps state");
+  if (conv_overlap(a, T, (T - 1) * x_row_stride + D, {new_state, bytes}, state))
+    return fail(GDN_ERR_VALUE, "an output overlaps another tensor");
   a.state = state;
   a.new_state = new_state;
   a.cu_seqlens = cu_seqlens;
@@ -494,6 +523,9 @@ int gdn_conv_pool(const void* x, int64_t x_batch_stride, int64_t x_row_stride, c
   if (!aligned(state_pool, 16)) return fail(GDN_ERR_VALUE, "state_pool must be 16-byte aligned");
   if (!aligned(in_slots, 4) || !aligned(out_slots, 4))
     return fail(GDN_ERR_VALUE, "slot arrays must be 4-byte aligned");
+  if (conv_overlap(a, B * T, (B - 1) * x_batch_stride + (T - 1) * x_row_stride + D,
+                   {state_pool, static_cast<size_t>(pool_size) * (W - 1) * D * 2}, nullptr))
+    return fail(GDN_ERR_VALUE, "an output overlaps another tensor");
   a.pool = state_pool;
   a.pool_size = pool_size;
   a.in_slots = in_slots;
@@ -507,6 +539,7 @@ static int check_ssm(const void* x, const void* B, const void* C, const float* A
   if (H <= 0 || G <= 0 || H % G != 0)
     return fail(GDN_ERR_VALUE, "num_heads (%lld) must be a positive multiple of num_groups (%lld)",
                 (long long)H, (long long)G);
+  if (H > 65536) return fail(GDN_ERR_VALUE, "num_heads must be at most 65536 (got %lld)", (long long)H);
   if (P != 64 && P != 128) return fail(GDN_ERR_VALUE, "head_dim must be 64 or 128 (got %lld)", (long long)P);
   if (Ns != 64 && Ns != 128)
     return fail(GDN_ERR_VALUE, "state_dim must be 64 or 128 (got %lld)", (long long)Ns);
@@ -527,8 +560,19 @@ static bool ssm_recurrent(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P)
   return T <= 16 * N && 2 * T <= (N * tiles > 128 ? N * tiles : 128);
 }
 
+// The scan's outputs against its inputs, `rows` tokens and states of `bytes` bytes.  (A call in two
+// launches reads x and a in the first while the second writes.)
+static bool ssm_overlap(const gdn::SsmArgs& p, int64_t rows, const void* states, const void* new_states, size_t bytes) {
+  const size_t x = static_cast<size_t>(rows) * p.H * p.P * 2, b = static_cast<size_t>(rows) * p.G * p.Ns * 2,
+               heads = static_cast<size_t>(p.H) * 4;
+  const Range w[2] = {{p.out, x}, {new_states, bytes}};
+  const Range r[8] = {{p.x, x}, {p.B, b}, {p.C, b}, {p.a, static_cast<size_t>(rows) * p.H * 2}, {states, bytes},
+                      {p.A_log, heads}, {p.dt_bias, heads}, {p.D, heads}};
+  return any_overlap(w, 2, r, 8);
+}
+
 size_t gdn_ssm_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P, int64_t Ns) {
-  if (T <= 0 || N <= 0 || H <= 0 || G <= 0 || H % G != 0 || (P != 64 && P != 128) || (Ns != 64 && Ns != 128) ||
+  if (T <= 0 || N <= 0 || T > 0x7fffffffLL - 64 || N > 0x7fffffffLL || H > 65536 || H <= 0 || G <= 0 || H % G != 0 || (P != 64 && P != 128) || (Ns != 64 && Ns != 128) ||
       ssm_recurrent(T, N, H, G, P))
     return 0;
   return gdn::ssm_chunked_workspace(T, N, H, G, P, Ns, sm_count());
@@ -555,6 +599,7 @@ int gdn_ssm(const void* x, const void* B, const void* C, const float* state, con
   p.x = x, p.B = B, p.C = C, p.state = state, p.A_log = A_log, p.a = a, p.dt_bias = dt_bias, p.D = D;
   p.cu_seqlens = cu_seqlens, p.out = output, p.new_state = new_state;
   p.T = T, p.N = N, p.H = H, p.G = G, p.P = P, p.Ns = Ns;
+  if (ssm_overlap(p, T, state, new_state, bytes)) return fail(GDN_ERR_VALUE, "an output overlaps another tensor");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (ssm_recurrent(T, N, H, G, P)) return cuda_status(gdn::launch_ssm_recurrent(p, st), "gdn_ssm launch");
   return cuda_status(gdn::launch_ssm_chunked(p, need ? workspace : nullptr, sm_count(), st), "gdn_ssm launch");
@@ -583,6 +628,9 @@ int gdn_ssm_pool(const void* x, const void* B, const void* C, const float* A_log
   p.T = T, p.N = batch, p.H = H, p.G = G, p.P = P, p.Ns = Ns, p.pool_size = pool_size;
   p.state_bf16 = state_dtype == GDN_STATE_BF16;
   p.no_state_update = (flags & GDN_POOL_NO_STATE_UPDATE) != 0;
+  if (ssm_overlap(p, batch * T, nullptr, state_pool,
+                  static_cast<size_t>(pool_size) * H * P * Ns * (p.state_bf16 ? 2 : 4)))
+    return fail(GDN_ERR_VALUE, "an output overlaps another tensor");
   return cuda_status(gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream)), "gdn_ssm_pool launch");
 }
 
@@ -614,6 +662,17 @@ int gdn_rms_norm(const void* x, int64_t x_stride, const void* weight, const void
   if (residual && overlap(residual, span, residual_out, static_cast<size_t>(rows) * D * 2) &&
       !(residual == residual_out && residual_stride == D))
     return fail(GDN_ERR_VALUE, "residual_out overlaps residual without being the same buffer");
+  // a row may be replaced by its own result (a thread reads its values before it writes them), no other
+  const size_t out_bytes = static_cast<size_t>(rows) * D * (scale ? 1 : 2), flat = static_cast<size_t>(rows) * D * 2;
+  const Range in[3] = {{x, (static_cast<size_t>(rows - 1) * strides[0] + D) * 2}, {residual, span},
+                       {gate, (static_cast<size_t>(rows - 1) * strides[2] + D) * 2}};
+  for (int i = 0; i < 3; ++i) {
+    const bool same = strides[i] == D;
+    if ((overlap(output, out_bytes, in[i].p, in[i].bytes) && !(same && !scale && output == in[i].p)) ||
+        (overlap(residual_out, flat, in[i].p, in[i].bytes) && !(same && residual_out == in[i].p)))
+      return fail(GDN_ERR_VALUE, "an output overlaps an input without being the same buffer");
+  }
+  if (overlap(output, out_bytes, residual_out, flat)) return fail(GDN_ERR_VALUE, "output overlaps residual_out");
   const gdn::NormArgs a{x, weight, residual, gate, output, scale, residual_out, x_stride, residual_stride,
                         gate_stride, rows, D, group, eps, dtype == GDN_F16,
                         (flags & GDN_NORM_GATE_FIRST) != 0};

@@ -113,3 +113,35 @@ def test_python_entry_points_reject_cpu_tensors(with_ext, monkeypatch):
                                      z(4, 2, 64, 64, dt=torch.float32), slots))):
         with pytest.raises(ValueError, match="CUDA"):
             fn(*args)
+
+
+@pytest.mark.parametrize("fn,args,over", [
+    ("gdn_conv", CONV, {}),  # (the output is x)
+    ("gdn_conv", CONV, dict(outs=arr(P, BASE + 2 * 64 * 9))),
+    ("gdn_conv", CONV, dict(xs=640, outs=arr(P, BASE + 2 * 128))),  # between the rows of x
+    ("gdn_conv", CONV, dict(outs=arr(P, 1 << 24))),  # new_state
+    ("gdn_conv", CONV, dict(outs=arr(P, 1 << 22, (1 << 22) + 640 - 16), widths=arr(ctypes.c_int64, 32, 32), n=2)),
+    ("gdn_conv_pool", CONV_POOL, dict(p_pool=1 << 24)),  # (the output is x)
+    ("gdn_conv_pool", CONV_POOL, dict(p_x=1 << 24)),  # (the output is the pool)
+    ("gdn_conv_pool", CONV_POOL, dict(p_x=1 << 24, p_pool=1 << 26, p_w=BASE + 128)),
+    ("gdn_ssm", SSM, {}),
+    ("gdn_ssm", SSM, dict(p_y=BASE + 10 * 4 * 64 * 2 - 16)),
+    ("gdn_ssm", SSM, dict(p_y=(1 << 26) + 1024)),
+    ("gdn_ssm", SSM, dict(p_y=1 << 25, p_C=(1 << 25) - 16)),
+    ("gdn_ssm_pool", SSM_POOL, dict(p_pool=1 << 24)),
+    ("gdn_ssm_pool", SSM_POOL, dict(p_y=1 << 24, p_pool=1 << 24)),
+    ("gdn_rms_norm", NORM, dict(p_out=BASE, xs=264)),
+    ("gdn_rms_norm", NORM, dict(p_out=BASE + 512)),
+    ("gdn_rms_norm", NORM, dict(p_out=BASE, p_scale=1 << 25)),
+    ("gdn_rms_norm", NORM, dict(p_out=(1 << 23) + 512)),
+    ("gdn_rms_norm", NORM, dict(p_x=1 << 24, p_ro=(1 << 24) + 512)),
+    ("gdn_rms_norm", NORM, dict(p_res=0, p_ro=0, p_gate=1 << 24, p_out=(1 << 24) + 16))])
+def test_outputs_that_overlap(fn, args, over):
+    rejects(fn, args, over, "overlaps")
+
+
+def test_sizes_past_any_tensor():
+    rejects("gdn_ssm", SSM, dict(H=1 << 57, G=1), "65536")
+    rejects("gdn_ssm_pool", SSM_POOL, dict(H=1 << 57, G=1), "65536")
+    assert N.lib().gdn_ssm_workspace_bytes(*[ctypes.c_int64(v) for v in (1 << 62, 1, 64, 1, 64, 128)]) == 0
+    assert N.lib().gdn_ssm_workspace_bytes(*[ctypes.c_int64(v) for v in (1 << 20, 1, 1 << 57, 1, 64, 128)]) == 0

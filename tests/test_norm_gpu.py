@@ -148,3 +148,26 @@ def test_refusals():
         norm.run_fp8(x[:, :136].contiguous(), w[:136].contiguous(), group_size=128)
     with pytest.raises(ValueError, match="group_size"):
         norm.run_fp8(x, w, group_size=64)
+
+
+@pytest.mark.parametrize("D", [72, 128, 1000, 4096, 8192])
+def test_in_place(D):
+    """The output or residual_out in the place of a contiguous input."""
+    from gdn_b200 import norm
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x, res, gate = (torch.randn(37, D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(3))
+    w = torch.rand(D, generator=g, device="cuda").to(torch.bfloat16)
+    want = norm.run(x, w)
+    y = x.clone()
+    assert norm.run(y, w, output=y).data_ptr() == y.data_ptr() and torch.equal(y, want)
+    want = norm.run(x, w, gate=gate)
+    y = gate.clone()
+    norm.run(x, w, gate=y, output=y)
+    assert torch.equal(y, want)
+    want, wr = norm.run(x, w, residual=res)
+    y, r = x.clone(), res.clone()
+    norm.run(y, w, residual=r, output=y, residual_out=r)
+    assert torch.equal(y, want) and torch.equal(r, wr)
+    y, r = x.clone(), res.clone()
+    norm.run(y, w, residual=r, output=r, residual_out=y)
+    assert torch.equal(r, want) and torch.equal(y, wr)
