@@ -882,7 +882,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t sb16 = sb >> 4;
     constexpr uint32_t kStage16 = L::kStage / 16, kBc16 = (L::OFF_ST + L::kX) / 16;
     auto wait = [&](int b, uint32_t parity) -> bool {
-      const bool done = mbar_test(&bars[b], parity) || wait_long(&bars[b], parity);
+      // (inline and without naps: every product waits for this warp; 4 % of the kernel's time)
+      const bool done = mbar_wait(&bars[b], parity, kTimeoutNs);
       tc_fence_after();
       return __all_sync(0xffffffffu, done);
     };
