@@ -320,12 +320,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) gdn_conv_kernel(ConvPa
 
 // T tokens of one sequence per (block row, thread): the state rows and the first
 // tokens are all loaded before any is used, and a thread writes only what it read.
-// Four channels a thread: 256 x 4 tokens x 8192 channels in 14.5 us (eight: 15.9; one token ahead
-// instead of four: 18.6), of which ~2 are the launch; the floor is 9.
-template <class T, int W, bool SILU, int kCh>
+// Four channels a thread, kAhead tokens loaded at once: 256 x 4 tokens x 8192 channels in 15.0 us
+// (eight channels: 15.9; kAhead 1: 19.0, 2: 18.4, 8: 17.8), 256 single tokens in 10.0 with kAhead 1
+// (11.6 with 4; eight channels 10.6; two sequences a thread 9.8, but 2.1 for one sequence instead of
+// 1.8), of which ~2 are the launch; the floors are 9 and 5.1.
+template <class T, int W, bool SILU, int kCh, int kAhead>
 __global__ void __launch_bounds__(kThreads) gdn_conv_pool_kernel(ConvParams p) {
   using R = Raw<kCh>;
-  constexpr int kAhead = 4;
   const int64_t c0 = (static_cast<int64_t>(blockIdx.x % p.col_blocks) * kThreads + threadIdx.x) * kCh;
   const int64_t n = blockIdx.x / p.col_blocks;
   if (c0 >= p.D) return;
@@ -387,8 +388,10 @@ cudaError_t launch(const ConvArgs& a, ConvParams p, cudaStream_t s) {
   }
   if (rows * p.col_blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const unsigned grid = static_cast<unsigned>(rows * p.col_blocks);
-  if (a.in_slots)
-    gdn_conv_pool_kernel<T, W, SILU, kPoolCh><<<grid, kThreads, 0, s>>>(p);
+  if (a.in_slots && a.T == 1)
+    gdn_conv_pool_kernel<T, W, SILU, kPoolCh, 1><<<grid, kThreads, 0, s>>>(p);
+  else if (a.in_slots)
+    gdn_conv_pool_kernel<T, W, SILU, kPoolCh, 4><<<grid, kThreads, 0, s>>>(p);
   else
     gdn_conv_kernel<T, W, SILU, kBatch, kDepth><<<grid, kThreads, 0, s>>>(p);
   return cudaGetLastError();
