@@ -12,7 +12,7 @@
 // 16-byte access per row) and walks a run of tokens with the window in registers, so each row
 // is read once per run plus W - 1 rows of the run before.  Rows ahead wait in shared memory
 // (cp.async): held in registers, 8 at a time, they left room for 3 blocks per SM and 3.8 TB/s;
-// like this 5.3-5.5 (bf16, W = 4: 7648 x 8192 in 46 us, 32768 x 6144 in 149 us; the copy peak
+// like this 5.4-5.7 (bf16, W = 4: 7648 x 8192 in 47 us, 32768 x 6144 in 140 us; the copy peak
 // gives 38 and 123).  Sums are in fp32, rounded once when stored; the states are copies of inputs.
 #include <algorithm>
 

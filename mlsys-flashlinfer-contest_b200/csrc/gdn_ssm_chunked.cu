@@ -37,8 +37,8 @@
 // step earlier, so no step waits for one to run, and warps meet through mbarriers only (they may
 // be in different steps).  What bounds the kernel is the compute warps' arithmetic and their
 // shared-memory accesses (issue slots ~50 % busy with 4.5 warps a scheduler), not HBM (29 %) or
-// the tensor pipe (30 %): 4 x 16384 tokens, 64 heads of 64, Ns 128: 670 us, 2.6 us a chunk;
-// with neither W nor M formed it would be 1.7 us.
+// the tensor pipe (30 %): 4 x 16384 tokens, 64 heads of 64, Ns 128: 641 us, 2.5 us a chunk;
+// with neither W nor M formed it would be 1.6 us.
 //
 // Few (sequence, head tile) pairs: sequences are cut into pieces of `seg` tokens.  A first
 // launch (STATE_ONLY) finds each piece's final state from zero and its decay; the second runs
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---- W of chunk c by quarters 0-1, in 16-byte pieces of x: a warp takes two tokens at a
     //      time (a token on 16 lanes), four times, 16 tokens apart.  (STATE_ONLY: every warp, twice,
-    //      32 apart.)  Shares of it for quarters 2-3 delayed M and cost 5-20 %. -----------------
+    //      32 apart.)  Shares of it for quarters 2-3 gained nothing or cost 5-20 %. -----------------
     const bool has_w = STATE_ONLY || quarter < 2;
     const int wt = (STATE_ONLY ? 2 * warp : (warp >> 2) * 4 + (warp & 1) * 2) + (lane >> 4);
     const int wblk = (lane >> 3) & 1;
@@ -1148,7 +1148,7 @@ struct Cut {
   int64_t slots = 0;  // at most so many pieces
 };
 
-// Times in units of one chunk of the second launch on one SM (~2.6 us): a chunk of the first,
+// Times in units of one chunk of the second launch on one SM (~2.5 us): a chunk of the first,
 // the start and end of a CTA, the state of one earlier piece, a launch.
 constexpr double kStateChunk = 0.4, kCta = 3.0, kJoin = 0.3, kLaunch = 1.5;
 

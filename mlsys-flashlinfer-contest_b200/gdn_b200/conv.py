@@ -68,8 +68,8 @@ def run(x, weight, bias, state, cu_seqlens, silu: bool = True, splits=None, outp
     weight [D, W] and bias [D] (or None) of x's dtype, W = 2, 3 or 4; state
     [N, W-1, D] or None (zeros); cu_seqlens [N+1] int64 (int32 is widened).
     ``splits``: channel counts (multiples of 8) of separate contiguous outputs.
-    Rows of no sequence are left as they were in given ``outputs``; a sequence of
-    length 0 keeps its state."""
+    Rows of no sequence are left as they were in given ``outputs``, which may not
+    overlap x or one another; a sequence of length 0 keeps its state."""
     cu_seqlens = _widen(cu_seqlens)
     ext = N.torch_ext()
     if ext is not None:

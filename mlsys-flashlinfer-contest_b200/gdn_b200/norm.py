@@ -81,7 +81,8 @@ def run(x, weight, eps: float = 1e-6, residual=None, gate=None, gate_first: bool
 
     x [..., D] bf16 or fp16, contiguous or 2D with a row stride; residual, gate of
     x's shape (not both); weight [D] of x's type; D a multiple of 8 up to 16384.
-    ``residual_out`` may be ``residual`` itself (in place)."""
+    ``output`` and ``residual_out`` may each be an input that is contiguous (in place),
+    but overlap nothing in part."""
     r = _run(x, weight, eps, residual, gate, gate_first, False, 0, output, residual_out)
     return tuple(r) if residual is not None else r[0]
 

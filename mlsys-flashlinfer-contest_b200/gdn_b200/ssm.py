@@ -51,7 +51,8 @@ def run(x, B, C, state, A_log, a, dt_bias, D, cu_seqlens, output=None, new_state
     x [T,H,P], B and C [T,G,state_dim], a [T,H] bf16; state [N,H,P,state_dim] fp32 or
     None (zeros); A_log, dt_bias [H] fp32; D [H] fp32 or None (no skip term);
     cu_seqlens [N+1] int64 (int32 is widened).  Rows of no sequence are left as they
-    were in a given ``output``; a sequence of length 0 keeps its state."""
+    were in a given ``output``, which may not overlap an input; a sequence of length 0
+    keeps its state."""
     cu_seqlens = _widen(cu_seqlens)
     ext = N.torch_ext()
     if ext is not None:
