@@ -14,10 +14,10 @@
 // exchange halves the values a lane still sums (9 shuffles for 8 rows instead of 40).  Gates
 // are computed a token on a lane.  State and sums are fp32; a bf16 pool is rounded once per
 // store.  Single tokens have their own instantiation, whose rows go from the raw load to the
-// store one by one; with several, the rows stay in registers and four tokens' sums are reduced at
+// store one by one; with several, the rows stay in registers and two or four tokens' sums are reduced at
 // once.  Measured with states larger than L2: single tokens, fp32, 256 x 64 heads of 64 x 128,
 // 161 us (1.02 of the copy peak; 174 with two blocks per SM instead of three); bf16 84 us (0.99;
-// 90 with three).  Four tokens, where the arithmetic counts: fp32 0.70, bf16 0.46.
+// 90 with three).  Four tokens, where the arithmetic counts: fp32 0.70, bf16 0.55.
 #include "gdn_internal.h"
 #include "gdn_vec16.cuh"
 
@@ -95,10 +95,11 @@ __device__ __forceinline__ void widen_x(const Vec<kN / 2>& v, float (&x)[kN]) {
 }
 
 // Ns = 64 or 128; BF16: storage of the state; PACKED: prompts by cu_seqlens (fp32 states
-// in and out) instead of a pool; ONE: a single token of each sequence; kU: rows a lane holds a
-// part of.
-template <int Ns, bool BF16, bool PACKED, bool ONE, int kU, int kBlocks>
+// in and out) instead of a pool; kTok: tokens whose inputs are loaded and whose sums are reduced
+// together (1: each sequence has a single token); kU: rows a lane holds a part of.
+template <int Ns, bool BF16, bool PACKED, int kTok, int kU, int kBlocks>
 __global__ void __launch_bounds__(kWarps * 32, kBlocks) gdn_ssm_recurrent_kernel(SsmArgs p) {
+  constexpr bool ONE = kTok == 1;
   constexpr int kVec = BF16 ? 8 : 4, kPairs = kVec / 2;
   constexpr int kLanes = Ns / kVec;        // lanes of a row: 8, 16 or 32
   constexpr int kRows = kU * 32 / kLanes;  // rows of a warp
@@ -143,7 +144,6 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks) gdn_ssm_recurrent_kernel
   const int64_t xpitch = p.H * p.P, bpitch = p.G * Ns;
 
   // kTok tokens at a time: their inputs are loaded together, and their dot products reduced together
-  constexpr int kTok = ONE ? 1 : 4;
   Vec<kPairs> Bn[kTok], Cn[kTok];
   Vec<kU / 2> xn[kTok];
   auto inputs = [&](int t0) {
@@ -256,22 +256,27 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks) gdn_ssm_recurrent_kernel
   }
 }
 
-template <int Ns, bool BF16, bool PACKED, bool ONE, int kU, int kBlocks>
+template <int Ns, bool BF16, bool PACKED, int kTok, int kU, int kBlocks>
 cudaError_t launch(const SsmArgs& a, cudaStream_t s) {
   constexpr int kRows = kU * 32 / (Ns / (BF16 ? 8 : 4));
   const int64_t units = a.N * a.H * (a.P / kRows);
   const int64_t blocks = (units + kWarps - 1) / kWarps;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  gdn_ssm_recurrent_kernel<Ns, BF16, PACKED, ONE, kU, kBlocks><<<static_cast<unsigned>(blocks), kWarps * 32, 0, s>>>(a);
+  gdn_ssm_recurrent_kernel<Ns, BF16, PACKED, kTok, kU, kBlocks><<<static_cast<unsigned>(blocks), kWarps * 32, 0, s>>>(a);
   return cudaGetLastError();
 }
 
-// (blocks per SM as measured: see above)
+// As measured (us; blocks per SM of single tokens: see above).  Two or four tokens at a time, bf16
+// states, 128 x 32 heads of 128 x 128: 57 | 81 for two tokens, 71 | 86 for three, 78 | 92 for four,
+// 132 | 150 for eight; fp32, 64 x 64 heads of 64 x 128: 48.5 | 53.5 for two, 58.2 | 55.9 for three,
+// 62.0 | 59.1 for four, 95 | 86 for eight.  Four rows a lane instead of eight, with more blocks: up
+// to 40 % slower.
 template <int Ns>
 cudaError_t by_form(const SsmArgs& a, cudaStream_t s) {
-  if (!a.in_slots) return launch<Ns, false, true, false, 8, 2>(a, s);
-  if (a.T == 1) return a.state_bf16 ? launch<Ns, true, false, true, 8, 2>(a, s) : launch<Ns, false, false, true, 8, 3>(a, s);
-  return a.state_bf16 ? launch<Ns, true, false, false, 8, 2>(a, s) : launch<Ns, false, false, false, 8, 2>(a, s);
+  if (!a.in_slots) return launch<Ns, false, true, 4, 8, 2>(a, s);
+  if (a.state_bf16) return a.T == 1 ? launch<Ns, true, false, 1, 8, 2>(a, s) : launch<Ns, true, false, 2, 8, 2>(a, s);
+  if (a.T <= 2) return a.T == 1 ? launch<Ns, false, false, 1, 8, 3>(a, s) : launch<Ns, false, false, 2, 8, 2>(a, s);
+  return launch<Ns, false, false, 4, 8, 2>(a, s);
 }
 
 }  // namespace

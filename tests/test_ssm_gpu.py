@@ -322,3 +322,22 @@ def test_long_sequences_among_hundreds():
         y, ya, S, Sa = L.scan_ref(*(m[k][a:b] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"], st[i])
         L.within(out[a:b], y, y_slack(ya, b - a))
         L.within(new[i], S, s_slack(Sa, b - a))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,P,G,Ns", [(4, 64, 2, 128), (3, 64, 1, 64), (2, 128, 1, 128), (2, 128, 2, 64)])
+@pytest.mark.parametrize("T", [2, 3, 5, 33])
+def test_pool_of_few_tokens(T, H, P, G, Ns, dtype):
+    from gdn_b200 import ssm
+    B = 3
+    m = make((B, T), H, P, G, Ns, seed=T + H)
+    pool = torch.randn(B + 2, H, P, Ns, device="cuda").to(dtype)
+    before = pool.clone()
+    ins, outs = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([4, 0, -1], [1, 3, 2]))
+    out = ssm.run_pool(m["x"], m["B"], m["C"], m["A_log"], m["a"], m["dt_bias"], m["D"], pool, ins, outs)
+    for i in range(B):
+        S0 = before[int(ins[i])] if ins[i] >= 0 else torch.zeros(H, P, Ns)
+        y, ya, S, Sa = L.scan_ref(*(m[k][i] for k in ("x", "B", "C", "a")), m["A_log"], m["dt_bias"], m["D"], S0)
+        L.within(out[i], y, f32_slack(ya, T))
+        L.within(pool[int(outs[i])], S, f32_slack(Sa, T))
+    assert torch.equal(pool[0], before[0]) and torch.equal(pool[4], before[4])
