@@ -6,12 +6,13 @@
 // the state at its start, every accumulator is transposed (a TMEM lane is a state row
 // (head, p)):
 //   G      = C B^T                                  [i, j]    (one product for all heads)
-//   M_h    = G e^{gamma_i - gamma_j} dt_j + D [i = j]  for j <= i      (bf16)
+//   M_h    = G e^{gamma_i - gamma_j} dt_j + D [i = j]  for j <= i
 //   (M X)^T = X^T M^T,  (C S)^T = S C^T             [row, i]
 //   y^T    = e^{gamma_i} (C S)^T + (M X)^T
 //   S     <- e^{gamma_63} S + W^T B,   W = e^{gamma_63 - gamma_j} dt_j x_j
-// Roundings: M and the S that C reads are bf16 operands (their errors, like the output's
-// own rounding, are 2^-8 of a term).  The state itself stays fp32 in registers for the whole
+// Roundings: M is an operand of two bf16 terms (16 bits: 2^-16 of a term, where the output's own
+// rounding is 2^-8; with one term the skip factor was rounded to bf16 and the outputs' error was 1.4
+// times that of their rounding), the S that C reads one bf16 term.  The state itself stays fp32 in registers for the whole
 // piece, and W enters its update as three bf16 terms (24 bits of mantissa; B is bf16
 // already): the final state is as exact as fp32 sums make it.  Two terms left 2.6e-6 of it.
 //
@@ -27,7 +28,8 @@
 // an infinite x would leak into earlier tokens, and 0 times a NaN weight into the other
 // head of a tile: x that is not finite is replaced by 0 as an operand and its row's outputs
 // from that token on are set to NaN; gates that are not finite are 0 in the operands and NaN in
-// the decays (e^gamma and the chunk's); tokens past the end are zeroed in x and B.
+// the decays (e^gamma and the chunk's), and so is a D that is not finite (or from 2^127 on) in its
+// head's e^gamma; tokens past the end are zeroed in x and B.
 //
 // Warp roles: warps 0-15 compute (four per TMEM lane quarter, each on a quarter of the
 // columns), warp 16 issues the MMAs, warp 17 the TMA loads and stores, warps 18-19 compute the
@@ -70,6 +72,7 @@ constexpr uint64_t kTimeoutNs = 2000000000ull;  // 2 s per wait, then give up
 constexpr int kStages = 3;
 constexpr int kRows = 128;  // state rows of a CTA
 constexpr int kTerms = 3;   // bf16 terms of W
+constexpr int kMTerms = 2;  // and of M
 
 // ---- TMEM columns ----------------------------------------------------------
 constexpr uint32_t TM_G = 0;     // lanes 64-127: G [i][j]
@@ -93,14 +96,19 @@ template <int P, int NS>
 struct Lay {
   static constexpr int kHeads = kRows / P;   // heads of a tile
   static constexpr int kKb = NS / 64;        // 64-column blocks of B and C
-  static constexpr uint32_t kX = 16384;      // [block 2][t 64][128 B]
-  static constexpr uint32_t kStage = kX + kKb * 16384;  // + [kb][B 64 rows | C 64 rows][128 B]
-  static constexpr uint32_t OFF_Z0 = 0;      // 2 KiB of zeros below the stages ...
-  static constexpr uint32_t OFF_ST = 2048;
-  static constexpr uint32_t OFF_Z1 = OFF_ST + kStages * kStage;  // ... and above
-  static constexpr uint32_t OFF_W = OFF_Z1 + 2048;    // the terms of W: [term 3][block 2][t 64][128 B]
-  static constexpr uint32_t OFF_M = OFF_W + kTerms * 16384;  // M of each head: [i 64][128 B]
-  static constexpr uint32_t OFF_G = OFF_M + 16384;    // tables [buffer][head][kGateFloats]
+  // B and C of a chunk wait for less long than its x, whose place its outputs take: two stages are
+  // enough for them where three do not fit
+  static constexpr int kBcStages = kHeads * kKb > 2 ? 2 : 3;
+  static constexpr uint32_t kX = 16384;         // [block 2][t 64][128 B]
+  static constexpr uint32_t kBc = kKb * 16384;  // [kb][B 64 rows | C 64 rows][128 B]
+  static constexpr uint32_t OFF_Z0 = 0;         // 2 KiB of zeros below the stages of x ...
+  static constexpr uint32_t OFF_X = 2048;
+  static constexpr uint32_t OFF_Z1 = OFF_X + kStages * kX;  // ... and above
+  static constexpr uint32_t OFF_BC = OFF_Z1 + 2048;
+  static constexpr uint32_t OFF_W = OFF_BC + kBcStages * kBc;  // the terms of W: [term 3][block 2][t 64][128 B]
+  static constexpr uint32_t OFF_M = OFF_W + kTerms * 16384;  // the terms of M: [term 2][head][i 64][128 B]
+  static constexpr uint32_t kM = kHeads * 8192;
+  static constexpr uint32_t OFF_G = OFF_M + (kMTerms * kM < 16384 ? 16384 : kMTerms * kM);  // tables [buffer][head][kGateFloats]
   static constexpr uint32_t OFF_DEC = OFF_G + kStages * 2 * kGateFloats * 4;  // [buffer][head]
   static constexpr uint32_t OFF_STEEP = OFF_DEC + 32;  // [buffer][head]: a bit per 16-block of G_V out of range
   static constexpr uint32_t OFF_BAD = OFF_STEEP + 32;  // first token whose x is not finite, by row
@@ -112,12 +120,12 @@ struct Lay {
   static constexpr uint32_t OFF_BAR = OFF_SKIP + 2 * kSkipHead;
   static constexpr uint32_t kBytes = OFF_BAR + 256 + 1024;
 };
-static_assert(Lay<64, 128>::kBytes <= 232448, "shared memory");
+static_assert(Lay<64, 128>::kBytes <= 232448 && Lay<128, 128>::kBytes <= 232448, "shared memory");
 
 enum : int {
-  B_BC = 0,                 // kStages: a chunk's B and C landed
+  B_BC = 0,                 // kBcStages: a chunk's B and C landed
   B_X = B_BC + kStages,     // kStages: its x landed and its tables are written
-  B_EMPTY = B_X + kStages,  // kStages: every product that reads the stage is done
+  B_EMPTY = B_X + kStages,  // kBcStages: every product that reads its B, C and x is done
   B_DONE = B_EMPTY + kStages,  // kStages: the compute warps are through with a chunk
   B_RDY_W = B_DONE + kStages, B_RDY_M,  // compute warps -> issue warp: operands of a chunk,
   B_RDY_S, B_RDY_D, B_RDY_D1,           // the state it starts from, its accumulators read
@@ -215,6 +223,9 @@ __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol
 
 // The long form of a wait, out of line: polls with short naps, gives up after kTimeoutNs.
 __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait_nap(bar, parity, kTimeoutNs); }
+
+// A skip factor that M can hold: any other makes every output of its head NaN.
+__device__ __forceinline__ bool usable_skip(float d) { return fabsf(d) < 0x1p127f; }
 
 struct Piece {
   int64_t seq, bos, eos;  // sequence (-1: none) and the piece's tokens
@@ -321,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                            const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ CUtensorMap tm_y,
                            const __grid_constant__ CUtensorMap tm_s, const __grid_constant__ CUtensorMap tm_n, const Params p) {
   using L = Lay<P, NS>;
-  constexpr int kHeads = L::kHeads, kKb = L::kKb;
+  constexpr int kHeads = L::kHeads, kKb = L::kKb, kBcStages = L::kBcStages;
   constexpr int kCols = NS / 4;  // state columns of a compute thread
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -383,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t x_bytes = kHeads == 2 && !two ? 8192u : 16384u;
   int bc_issued = 0, x_issued = 0;  // (load thread)
   auto load_bc = [&](int c) {
-    const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
-    uint8_t* bc = smem + L::OFF_ST + st * L::kStage + L::kX;
+    const int st = c % kBcStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
+    uint8_t* bc = smem + L::OFF_BC + st * L::kBc;
     mbar_arrive_expect_tx(&bars[B_BC + st], kKb * (STATE_ONLY ? 8192u : 16384u));
 #pragma unroll
     for (int kb = 0; kb < kKb; ++kb) {
@@ -395,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   auto load_x = [&](int c) {
     const int st = c % kStages, tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
-    uint8_t* xs = smem + L::OFF_ST + st * L::kStage;
+    uint8_t* xs = smem + L::OFF_X + st * L::kX;
     mbar_arrive_expect_tx(&bars[B_X + st], x_bytes);
     tma_load_3d(xs, &tm_x, &bars[B_X + st], 0, h0, tok);
     if (P == 128)
@@ -426,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     for (int c = 0; c < min(n, kStages); ++c) {
-      load_bc(c);
+      if (c < kBcStages) load_bc(c);
       load_x(c);
     }
     if (!STATE_ONLY) prefetch_tmap(&tm_y);
@@ -437,15 +448,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (tid < kRows) first_bad[tid] = 0x7fffffff;
   if (!STATE_ONLY) {
-    // zeros: the blocks beside the stages, M's columns above the diagonal
+    // zeros: the blocks beside the stages of x
     for (int i = tid; i < 128; i += kThreads) {
       sts128(sb + L::OFF_Z0 + 16 * i, 0u, 0u, 0u, 0u);
       sts128(sb + L::OFF_Z1 + 16 * i, 0u, 0u, 0u, 0u);
     }
     float skip[2] = {0.f, 0.f};
     if (p.D) {
-      skip[0] = p.D[h0];
-      if (two) skip[1] = p.D[h0 + 1];
+      skip[0] = usable_skip(p.D[h0]) ? p.D[h0] : 0.f;
+      if (two) skip[1] = usable_skip(p.D[h0 + 1]) ? p.D[h0 + 1] : 0.f;
     }
     for (int i = tid; i < 18 * 16; i += kThreads) {
       const int d = i / 16 - 1, j = i % 16;
@@ -457,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (kHeads == 2 && !two)  // the absent head's x
     for (int i = tid; i < kStages * 512; i += kThreads)
-      sts128(sb + L::OFF_ST + (i >> 9) * L::kStage + 8192 + 16 * (i & 511), 0u, 0u, 0u, 0u);
+      sts128(sb + L::OFF_X + (i >> 9) * L::kX + 8192 + 16 * (i & 511), 0u, 0u, 0u, 0u);
   // (gate warps: head gh, two tokens a lane)
   const int gh = warp - kGateWarp;
   const bool live = warp >= kGateWarp && (gh == 0 || (kHeads == 2 && two));
@@ -471,7 +482,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
   float negA = 0.f, bias = 0.f;
+  bool skip_ok = true;
   if (live) {
+    skip_ok = !p.D || usable_skip(p.D[h0 + gh]);
     negA = -expf(p.A_log[h0 + gh]) * kLog2e;
     bias = p.dt_bias[h0 + gh];
     load_gates(0);
@@ -526,9 +539,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < kCols; ++i) s[i] = 0.f;
     }
-    if (!STATE_ONLY) {  // M's columns above the diagonal are zero from here on
+    if (!STATE_ONLY) {  // the blocks of M that no warp writes (rows 0-31, columns 32-63) are zero from here on
       if (state_in) named_sync(kComputeBar, kComputeThreads);  // (every thread has its state)
-      for (int i = tid; i < 1024; i += kComputeThreads) sts128(sb + L::OFF_M + 16 * i, 0u, 0u, 0u, 0u);
+      for (int i = tid; i < static_cast<int>(kMTerms * kHeads * 128); i += kComputeThreads)
+        sts128(sb + L::OFF_M + (i >> 7) * 8192 + sw128_off(i >> 2 & 31, 4 + (i & 3)), 0u, 0u, 0u, 0u);
       fence_async_smem();
       named_sync(kComputeBar, kComputeThreads);
     }
@@ -576,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t woff = wblk * 8192 + sw128_off(wt, lane & 7);
     constexpr int kStride = STATE_ONLY ? 32 : 16, kCount = kChunk / kStride;
     auto make_w = [&](int c, int st, uint32_t st_par) {
-      const uint32_t xs = sb + L::OFF_ST + st * L::kStage + woff;
+      const uint32_t xs = sb + L::OFF_X + st * L::kX + woff;
       const int Lc = static_cast<int>(min(static_cast<int64_t>(kChunk), Ltot - static_cast<int64_t>(c) * kChunk));
       wait(B_X + st, st_par);
       uint4 x[kCount];
@@ -587,14 +601,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         w[k] = table(st, kHeads == 2 ? wblk : 0)[G_W + wt + kStride * k];
       }
       if (Lc < kChunk) {  // tokens past the end: x and B become zero
-        wait(B_BC + st, st_par);
+        wait(B_BC + c % kBcStages, static_cast<uint32_t>((c / kBcStages) & 1));
+        const uint32_t bs = sb + L::OFF_BC + c % kBcStages * L::kBc + wblk * 8192 + woff;  // (blocks 16 KiB apart)
 #pragma unroll
         for (int k = 0; k < kCount; ++k)
           if (wt + kStride * k >= Lc) {
             x[k] = make_uint4(0, 0, 0, 0);
             sts128(xs + k * (kStride * 128), 0u, 0u, 0u, 0u);
-            if (wblk < kKb)  // (block wblk of B lies 16 KiB apart, of x 8 KiB)
-              sts128(xs + L::kX + wblk * 8192 + k * (kStride * 128), 0u, 0u, 0u, 0u);
+            if (wblk < kKb) sts128(bs + k * (kStride * 128), 0u, 0u, 0u, 0u);
           }
       }
       if (c > 0) wait_ds(c - 1);  // W is free
@@ -662,7 +676,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld16(tl + TM_G + r0, v);
       tmem_wait_ld();
       reg_fence(v);
-      uint32_t m[8];
+      uint32_t m[8], ml[8];
+      // the rounded value, then what it left (as W's terms)
+      auto split = [&](float2 q, uint32_t& hi, uint32_t& lo) {
+        hi = pack_bf16x2(q.x, q.y);
+        const float2 r = __ffma2_rn(make_float2(bf16_lo(hi), bf16_hi(hi)), make_float2(-1.f, -1.f), q);
+        lo = pack_bf16x2(r.x, r.y);
+      };
       if constexpr (kBelow) {
         float u[16];
         load16(tb + G_U + r0, u);
@@ -670,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = 0; k < 8; ++k) {
           const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
                                       make_float2(r, r));
-          m[k] = pack_bf16x2(q.x, q.y);
+          split(q, m[k], ml[k]);
         }
       } else {
         const int md = min(max(mi - r0, -1), 16) + 1;  // row of the mask and skip tables
@@ -697,16 +717,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k4 = 0; k4 < 2; ++k4) {
           const uint4 a = mask[k4];
-          m[4 * k4] = pack_bf16x2(q[4 * k4].x, q[4 * k4].y) & a.x;
-          m[4 * k4 + 1] = pack_bf16x2(q[4 * k4 + 1].x, q[4 * k4 + 1].y) & a.y;
-          m[4 * k4 + 2] = pack_bf16x2(q[4 * k4 + 2].x, q[4 * k4 + 2].y) & a.z;
-          m[4 * k4 + 3] = pack_bf16x2(q[4 * k4 + 3].x, q[4 * k4 + 3].y) & a.w;
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            split(q[4 * k4 + k], m[4 * k4 + k], ml[4 * k4 + k]);
+            m[4 * k4 + k] &= aw[k];
+            ml[4 * k4 + k] &= aw[k];
+          }
         }
       }
 #pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2)
-        sts128_op(sb + L::OFF_M + head * 8192 + sw128_off(mi, 2 * cb + c2), m[4 * c2], m[4 * c2 + 1], m[4 * c2 + 2],
-                  m[4 * c2 + 3]);
+      for (int c2 = 0; c2 < 2; ++c2) {
+        const uint32_t dst = sb + L::OFF_M + head * 8192 + sw128_off(mi, 2 * cb + c2);
+        sts128_op(dst, m[4 * c2], m[4 * c2 + 1], m[4 * c2 + 2], m[4 * c2 + 3]);
+        sts128_op(dst + L::kM, ml[4 * c2], ml[4 * c2 + 1], ml[4 * c2 + 2], ml[4 * c2 + 3]);
+      }
     };
     auto make_m = [&](int c, int st, uint32_t st_par) {
       wait(B_X + st, st_par);  // (the tables)
@@ -770,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t left = Ltot - static_cast<int64_t>(c) * kChunk;
       if (!row_live) return;
       if (left >= kChunk) {
-        const uint32_t ys = sb + L::OFF_ST + st * L::kStage + ysm;
+        const uint32_t ys = sb + L::OFF_X + st * L::kX + ysm;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {  // token k or k ^ 4 of eight: its row, and its swizzle
           const uint32_t t = odd ? k ^ 4 : k;
@@ -880,17 +905,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t leader = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);  // (uniform)
     const uint32_t sb16 = sb >> 4;
-    constexpr uint32_t kStage16 = L::kStage / 16, kBc16 = (L::OFF_ST + L::kX) / 16;
+    constexpr uint32_t kBcSize16 = L::kBc / 16, kBc16 = L::OFF_BC / 16;
     auto wait = [&](int b, uint32_t parity) -> bool {
       // (inline and without naps: every product waits for this warp; 4 % of the kernel's time)
       const bool done = mbar_wait(&bars[b], parity, kTimeoutNs);
       tc_fence_after();
       return __all_sync(0xffffffffu, done);
     };
-    // (st: the chunk's stage)
-    auto mma_g = [&](int st, uint32_t par) -> bool {
-      if (!wait(B_BC + st, par)) return false;
-      const uint32_t bc = sb16 + kBc16 + st * kStage16;
+    // (bst: the stage of the chunk's B and C, xst: of its x)
+    auto mma_g = [&](int bst, uint32_t par) -> bool {
+      if (!wait(B_BC + bst, par)) return false;
+      const uint32_t bc = sb16 + kBc16 + bst * kBcSize16;
 #pragma unroll
       for (int ks = 0; ks < NS / 16; ++ks) {
         const uint64_t d = sdesc_sw128_f(bc + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16, 16, 1024);
@@ -899,8 +924,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit_by(leader, &bars[B_G]);
       return true;
     };
-    auto mma_ds = [&](int c, int st) {
-      const uint32_t d = tm + TM_DS + (STATE_ONLY ? 128 * (c & 1) : 0), bc = sb16 + kBc16 + st * kStage16;
+    auto mma_ds = [&](int c, int bst) {
+      const uint32_t d = tm + TM_DS + (STATE_ONLY ? 128 * (c & 1) : 0), bc = sb16 + kBc16 + bst * kBcSize16;
 #pragma unroll
       for (int part = 0; part < kTerms; ++part)
 #pragma unroll
@@ -909,13 +934,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sdesc_sw128_f(bc + ks * 128, 16384, 1024), idesc_ds, part > 0 || ks > 0);
       commit_by(leader, &bars[B_DS + (STATE_ONLY ? c & 1 : 0)]);
     };
-    auto mma_pv = [&](int c, int st) {
-      const uint32_t xo = L::OFF_ST + st * L::kStage;
+    auto mma_pv = [&](int c, int xst) {
+      const uint32_t xo = L::OFF_X + xst * L::kX;
 #pragma unroll
       for (int head = 0; head < kHeads; ++head)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          const uint64_t b = sdesc_sw128_f(sb16 + (L::OFF_M + head * 8192 + ks * 32) / 16, 16, 1024);
           // rows 0-63 and 64-127 of X^T are two blocks of 64; with two heads, the block of the
           // other head is 2 KiB of zeros, so that each head's M meets its own x only
           uint32_t start = xo + ks * 2048, lbo = 8192;
@@ -924,12 +948,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             lbo = start + 8192 - L::OFF_Z0;
             start = L::OFF_Z0;
           }
-          mma_ss_by(leader, tm + TM_PV + 64 * (c & 1), sdesc_sw128_f(sb16 + start / 16, lbo, 1024), b, idesc_pv, head > 0 || ks > 0);
+          const uint64_t a = sdesc_sw128_f(sb16 + start / 16, lbo, 1024);
+#pragma unroll
+          for (int term = 0; term < kMTerms; ++term)
+            mma_ss_by(leader, tm + TM_PV + 64 * (c & 1), a,
+                      sdesc_sw128_f(sb16 + (L::OFF_M + term * L::kM + head * 8192 + ks * 32) / 16, 16, 1024), idesc_pv,
+                      head > 0 || ks > 0 || term > 0);
         }
       commit_by(leader, &bars[B_PV + (c & 1)]);
     };
-    auto mma_qs = [&](int c, int st) {
-      const uint32_t bc = sb16 + kBc16 + st * kStage16;
+    auto mma_qs = [&](int c, int bst) {
+      const uint32_t bc = sb16 + kBc16 + bst * kBcSize16;
 #pragma unroll
       for (int ks = 0; ks < NS / 16; ++ks)
         mma_ts_by(leader, tm + TM_QS + 64 * (c & 1), tm + TM_SB + 8 * ks,
@@ -937,39 +966,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit_by(leader, &bars[B_QS + (c & 1)]);
     };
     bool ok = STATE_ONLY || mma_g(0, 0);
-    // stages of chunks c, c + 1 and c + 2, and the parities of c's and of c + 2's
-    int s0 = kStages - 1, s1 = 0, s2 = 1;
-    uint32_t par0 = 1, par2 = 0;
-    for (int c = -1; ok && c < n; ++c) {
+    // stages of chunk c + 1 (of B and C, of x) and of chunk c + 2 (of B and C, with its parity)
+    int b1 = 0, x1 = 0, b2 = 1;
+    uint32_t par1 = 0, par2 = 0;
+    for (int c = -1; ok && c + 1 < n; ++c) {
       const uint32_t next = static_cast<uint32_t>((c + 1) & 1);
       if (STATE_ONLY) {
-        if (c + 1 == n) break;
         // (the buffer of W^T B was read in the update of chunk c - 1)
         if (c >= 1 && !(ok = wait(B_DONE + (c - 1) % kStages, static_cast<uint32_t>(((c - 1) / kStages) & 1)))) break;
-        if (!(ok = wait(B_BC + s1, s1 == 0 ? par0 ^ 1u : par0))) break;
+        if (!(ok = wait(B_BC + b1, par1))) break;
         if (!(ok = wait(B_RDY_W, next))) break;
-        mma_ds(c + 1, s1);
-        commit_by(leader, &bars[B_EMPTY + s1]);
+        mma_ds(c + 1, b1);
+        commit_by(leader, &bars[B_EMPTY + b1]);
       } else {
         // the outputs of chunk c - 1 have read the buffers that chunk c + 1 takes
         if (c >= 1 && !(ok = wait(B_RDY_D + static_cast<int>(next), static_cast<uint32_t>(((c - 1) >> 1) & 1)))) break;
-        if (c + 1 == n) break;
         if (!(ok = wait(B_RDY_M, next))) break;
-        if (c + 2 < n && !(ok = mma_g(s2, par2))) break;
+        // (with two stages of B and C, chunk c + 2's are just being loaded)
+        if (kBcStages == 3 && c + 2 < n && !(ok = mma_g(b2, par2))) break;
         if (!(ok = wait(B_RDY_W, next))) break;
-        mma_pv(c + 1, s1);
+        mma_pv(c + 1, x1);
         if (!(ok = wait(B_RDY_S, next))) break;  // the update of chunk c has read W^T B
-        mma_ds(c + 1, s1);
-        mma_qs(c + 1, s1);
-        commit_by(leader, &bars[B_EMPTY + s1]);
+        mma_ds(c + 1, b1);
+        mma_qs(c + 1, b1);
+        commit_by(leader, &bars[B_EMPTY + b1]);
+        if (kBcStages == 2 && c + 2 < n && !(ok = mma_g(b2, par2))) break;
       }
-      s0 = s1;
-      s1 = s2;
-      if (s0 == 0) par0 ^= 1u;
-      if (++s2 == kStages) {
-        s2 = 0;
+      b1 = b2;
+      par1 = par2;
+      if (++b2 == kBcStages) {
+        b2 = 0;
         par2 ^= 1u;
       }
+      if (++x1 == kStages) x1 = 0;
     }
     commit_by(leader, &bars[B_END]);
     failed = !wait(B_END, 0) || !ok;
@@ -1025,8 +1054,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             make_float2(dt[0] * ex2_ftz(first - gt[0]), dt[1] * ex2_ftz(first - gt[1]));
         *reinterpret_cast<float2*>(tb + G_W + 2 * lane) = make_float2(dt[0] * ex2_ftz(rest[0]), dt[1] * ex2_ftz(rest[1]));
         const float nan = __int_as_float(0x7fc00000);
+        const int fy = skip_ok ? fb : 0;  // first output that is not finite
         *reinterpret_cast<float2*>(tb + G_EG + 2 * lane) =
-            make_float2(2 * lane >= fb ? nan : ex2_ftz(gt[0]), 2 * lane + 1 >= fb ? nan : ex2_ftz(gt[1]));
+            make_float2(2 * lane >= fy ? nan : ex2_ftz(gt[0]), 2 * lane + 1 >= fy ? nan : ex2_ftz(gt[1]));
         if (lane == 0) {
           decs[buf * 2 + gh] = fb < 64 ? nan : ex2_ftz(g63);
           steep[buf * 2 + gh] = (far & 1u) | (far >> 7 & 2u) | (far >> 14 & 4u) | (far >> 21 & 8u);
@@ -1043,18 +1073,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ======================= TMA load and store thread =========================
     bool ok = true;
     for (int c = 0; ok && c < n; ++c) {
-      const int st = c % kStages;
+      const int st = c % kStages, bst = c % kBcStages;
       const uint32_t par = static_cast<uint32_t>((c / kStages) & 1);
-      if (c + kStages < n) {
-        if (!(ok = mbar_wait(&bars[B_EMPTY + st], par, kTimeoutNs))) break;
-        load_bc(c + kStages);
-        if (STATE_ONLY) load_x(c + kStages);
+      if (c + kBcStages < n) {
+        if (!(ok = mbar_wait(&bars[B_EMPTY + bst], static_cast<uint32_t>((c / kBcStages) & 1), kTimeoutNs))) break;
+        load_bc(c + kBcStages);
+        if (STATE_ONLY && c + kStages < n) load_x(c + kStages);
       }
       if (STATE_ONLY) continue;
       if (!(ok = mbar_wait(&bars[B_DONE + st], par, kTimeoutNs))) break;
       if (Ltot - static_cast<int64_t>(c) * kChunk >= kChunk) {  // the outputs, where x was
         const int tok = static_cast<int>(bos + static_cast<int64_t>(c) * kChunk);
-        const uint8_t* ys = smem + L::OFF_ST + st * L::kStage;
+        const uint8_t* ys = smem + L::OFF_X + st * L::kX;
         tma_store_3d(&tm_y, ys, 0, h0, tok);
         if (P == 128)
           tma_store_3d(&tm_y, ys + 8192, 64, h0, tok);
@@ -1069,8 +1099,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // no load may be in flight, and no store may still read, when the CTA ends
     bulk_wait_read_all();
-    for (int c = max(0, bc_issued - kStages); c < bc_issued; ++c)
-      if (!mbar_wait(&bars[B_BC + c % kStages], static_cast<uint32_t>((c / kStages) & 1), kTimeoutNs)) ok = false;
+    for (int c = max(0, bc_issued - kBcStages); c < bc_issued; ++c)
+      if (!mbar_wait(&bars[B_BC + c % kBcStages], static_cast<uint32_t>((c / kBcStages) & 1), kTimeoutNs)) ok = false;
     for (int c = max(0, x_issued - kStages); c < x_issued; ++c)
       if (!mbar_wait(&bars[B_X + c % kStages], static_cast<uint32_t>((c / kStages) & 1), kTimeoutNs)) ok = false;
     failed = !ok;
