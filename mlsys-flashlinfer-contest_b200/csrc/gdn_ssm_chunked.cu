@@ -10,11 +10,13 @@
 //   (M X)^T = X^T M^T,  (C S)^T = S C^T             [row, i]
 //   y^T    = e^{gamma_i} (C S)^T + (M X)^T
 //   S     <- e^{gamma_63} S + W^T B,   W = e^{gamma_63 - gamma_j} dt_j x_j
-// Roundings: M is an operand of two bf16 terms (16 bits: 2^-16 of a term, where the output's own
-// rounding is 2^-8; with one term the skip factor was rounded to bf16 and the outputs' error was 1.4
-// times that of their rounding), the S that C reads one bf16 term.  The state itself stays fp32 in registers for the whole
-// piece, and W enters its update as three bf16 terms (24 bits of mantissa; B is bf16
-// already): the final state is as exact as fp32 sums make it.  Two terms left 2.6e-6 of it.
+// Roundings: M and the S that C reads are operands of two bf16 terms, the rounded value and what it
+// left (16 bits: 2^-16 of a term, where the output's own rounding is 2^-8; with one term each the
+// outputs' error was 1.4 times that of their rounding, and the skip factor itself was rounded).  The state
+// itself stays fp32 in registers for the whole piece, and W enters its update as three bf16 terms (24
+// bits of mantissa; B is bf16 already): the final state is as exact as fp32 sums make it.  Two terms left
+// 2.6e-6 of it.  The second terms cost 0-9 % of the time (one prompt of 8192 tokens, 64 heads of 64: 134
+// -> 136 us; four of 8192 327 -> 353; 16 ragged ones, heads of 128: 107 -> 109).
 //
 // The decays between a row and the columns of a 16-column block are r_i u_j.  Below the
 // diagonal u_j = dt_j e^{gamma_top - gamma_j} (a table, top = the block's last column) and
@@ -24,12 +26,15 @@
 // exponential.  The mask and the skip term D of a row come from tables in shared memory (a mask
 // word per two columns, applied to the packed bf16 values, so that it also hides a NaN).
 //
+// Two heads of a tile: M X is one product of N = 128, [M_0 | M_1] against the x of both, of which each
+// row reads its own head's 64 columns.  Half of it is thrown away, as it would be with a product of
+// zeros for each head, but no head's M meets the other's x: what is not finite in one (D, an
+// overflow) stays there, and it is half as many MMAs to issue.
+//
 // Values that are not finite stay where the recurrence puts them.  A masked factor 0 times
-// an infinite x would leak into earlier tokens, and 0 times a NaN weight into the other
-// head of a tile: x that is not finite is replaced by 0 as an operand and its row's outputs
-// from that token on are set to NaN; gates that are not finite are 0 in the operands and NaN in
-// the decays (e^gamma and the chunk's), and so is a D that is not finite (or from 2^127 on) in its
-// head's e^gamma; tokens past the end are zeroed in x and B.
+// an infinite x would leak into earlier tokens: x that is not finite is replaced by 0 as an operand and
+// its row's outputs from that token on are set to NaN; gates that are not finite are 0 in the operands
+// and NaN in the decays (e^gamma and the chunk's); tokens past the end are zeroed in x and B.
 //
 // Warp roles: warps 0-15 compute (four per TMEM lane quarter, each on a quarter of the
 // columns), warp 16 issues the MMAs, warp 17 the TMA loads and stores, warps 18-19 compute the
@@ -77,9 +82,9 @@ constexpr int kMTerms = 2;  // and of M
 // ---- TMEM columns ----------------------------------------------------------
 constexpr uint32_t TM_G = 0;     // lanes 64-127: G [i][j]
 constexpr uint32_t TM_DS = 64;   // W^T B [row][n] (STATE_ONLY: two buffers of 128 columns)
-constexpr uint32_t TM_QS = 192;  // (C S)^T [row][i], two buffers of 64 columns
-constexpr uint32_t TM_PV = 320;  // (M X)^T [row][i], two buffers of 64 columns
-constexpr uint32_t TM_SB = 448;  // S as bf16 [row][n]: A operand
+constexpr uint32_t TM_QS = 192;  // (C S)^T [row][i]
+constexpr uint32_t TM_PV = 256;  // (M X)^T [row][head of M][i]
+constexpr uint32_t TM_SB = 384;  // the two bf16 terms of S [term][row][n]: A operands, 64 columns each
 constexpr uint32_t kTmemCols = 512;
 
 // ---- per-token tables (floats) of one head and chunk ------------------------
@@ -96,15 +101,13 @@ template <int P, int NS>
 struct Lay {
   static constexpr int kHeads = kRows / P;   // heads of a tile
   static constexpr int kKb = NS / 64;        // 64-column blocks of B and C
-  // B and C of a chunk wait for less long than its x, whose place its outputs take: two stages are
+  // B and C of a chunk are done with before its x, whose place its outputs take: two stages are
   // enough for them where three do not fit
   static constexpr int kBcStages = kHeads * kKb > 2 ? 2 : 3;
   static constexpr uint32_t kX = 16384;         // [block 2][t 64][128 B]
   static constexpr uint32_t kBc = kKb * 16384;  // [kb][B 64 rows | C 64 rows][128 B]
-  static constexpr uint32_t OFF_Z0 = 0;         // 2 KiB of zeros below the stages of x ...
-  static constexpr uint32_t OFF_X = 2048;
-  static constexpr uint32_t OFF_Z1 = OFF_X + kStages * kX;  // ... and above
-  static constexpr uint32_t OFF_BC = OFF_Z1 + 2048;
+  static constexpr uint32_t OFF_X = 0;
+  static constexpr uint32_t OFF_BC = OFF_X + kStages * kX;
   static constexpr uint32_t OFF_W = OFF_BC + kBcStages * kBc;  // the terms of W: [term 3][block 2][t 64][128 B]
   static constexpr uint32_t OFF_M = OFF_W + kTerms * 16384;  // the terms of M: [term 2][head][i 64][128 B]
   static constexpr uint32_t kM = kHeads * 8192;
@@ -128,9 +131,8 @@ enum : int {
   B_EMPTY = B_X + kStages,  // kBcStages: every product that reads its B, C and x is done
   B_DONE = B_EMPTY + kStages,  // kStages: the compute warps are through with a chunk
   B_RDY_W = B_DONE + kStages, B_RDY_M,  // compute warps -> issue warp: operands of a chunk,
-  B_RDY_S, B_RDY_D, B_RDY_D1,           // the state it starts from, its accumulators read
-  // products done (two where a chunk's may complete before every warp has met the one before)
-  B_G, B_DS, B_DS1, B_PV, B_PV1, B_QS, B_QS1, B_END,
+  B_RDY_S, B_RDY_D,                     // W^T B of the chunk before read, its other accumulators read
+  B_G, B_DS, B_DS1, B_PV, B_QS, B_END,  // products done (two of W^T B with STATE_ONLY: its buffers)
   B_STATE,  // the initial state landed
   kNumBars
 };
@@ -205,6 +207,18 @@ __device__ __forceinline__ void commit_by(uint32_t leader, uint64_t* bar) {
       "r"(leader)
       : "memory");
 }
+// What two values leave when their bf16 roundings (packed in `hi`) are taken off: x - hi is exact in fp32.
+__device__ __forceinline__ float2 minus_bf16x2(float2 x, uint32_t hi) {
+  float2 r;
+  asm("{\n\t.reg .b16 l, h, m;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "mov.b16 m, 0xBF80;\n\t"
+      "fma.rn.f32.bf16 %0, l, m, %3;\n\t"
+      "fma.rn.f32.bf16 %1, h, m, %4;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(hi), "f"(x.x), "f"(x.y));
+  return r;
+}
 // One lane of the (converged) warp.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
@@ -223,9 +237,6 @@ __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol
 
 // The long form of a wait, out of line: polls with short naps, gives up after kTimeoutNs.
 __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait_nap(bar, parity, kTimeoutNs); }
-
-// A skip factor that M can hold: any other makes every output of its head NaN.
-__device__ __forceinline__ bool usable_skip(float d) { return fabsf(d) < 0x1p127f; }
 
 struct Piece {
   int64_t seq, bos, eos;  // sequence (-1: none) and the piece's tokens
@@ -423,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kLoadWarp && lane == 0) {
     for (int i = 0; i < kNumBars; ++i)
       mbar_init(&bars[i], i == B_RDY_W ? (STATE_ONLY ? kComputeWarps : kComputeWarps / 2) : i == B_RDY_M ? (kHeads == 2 ? 8 : 6)
-                         : (i == B_RDY_S || i == B_RDY_D || i == B_RDY_D1 || (i >= B_DONE && i < B_DONE + kStages)) ? kComputeWarps
+                         : (i == B_RDY_S || i == B_RDY_D || (i >= B_DONE && i < B_DONE + kStages)) ? kComputeWarps
                          : i >= B_X && i < B_EMPTY ? 1 + kHeads : 1);
     fence_mbar_init();
     *abort_flag = 0u;
@@ -448,15 +459,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (tid < kRows) first_bad[tid] = 0x7fffffff;
   if (!STATE_ONLY) {
-    // zeros: the blocks beside the stages of x
-    for (int i = tid; i < 128; i += kThreads) {
-      sts128(sb + L::OFF_Z0 + 16 * i, 0u, 0u, 0u, 0u);
-      sts128(sb + L::OFF_Z1 + 16 * i, 0u, 0u, 0u, 0u);
-    }
     float skip[2] = {0.f, 0.f};
     if (p.D) {
-      skip[0] = usable_skip(p.D[h0]) ? p.D[h0] : 0.f;
-      if (two) skip[1] = usable_skip(p.D[h0 + 1]) ? p.D[h0 + 1] : 0.f;
+      skip[0] = p.D[h0];
+      if (two) skip[1] = p.D[h0 + 1];
     }
     for (int i = tid; i < 18 * 16; i += kThreads) {
       const int d = i / 16 - 1, j = i % 16;
@@ -482,9 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
   float negA = 0.f, bias = 0.f;
-  bool skip_ok = true;
   if (live) {
-    skip_ok = !p.D || usable_skip(p.D[h0 + gh]);
     negA = -expf(p.A_log[h0 + gh]) * kLog2e;
     bias = p.dt_bias[h0 + gh];
     load_gates(0);
@@ -563,21 +567,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    auto publish_state = [&]() {  // S as the bf16 A operand of (C S)^T
-      const uint32_t dst = tl + TM_SB;
-      uint32_t w[kCols / 2];
-#pragma unroll
-      for (int i = 0; i < kCols / 2; ++i) w[i] = pack_bf16x2(s[2 * i], s[2 * i + 1]);
-      if constexpr (kCols == 32)
-        tmem_st16u(dst + 16 * cq, w);
-      else
-        tmem_st8u(dst + 8 * cq, w);
-      tmem_wait_st();
-      signal(B_RDY_S, false);
+    // a value as bf16 terms: the rounded value, then what it left
+    auto split = [](float2 q, uint32_t& hi, uint32_t& lo) {
+      hi = pack_bf16x2(q.x, q.y);
+      const float2 r = minus_bf16x2(q, hi);
+      lo = pack_bf16x2(r.x, r.y);
     };
-    if (!STATE_ONLY) publish_state();
-    // products that come in two buffers by the chunk's parity
-    auto wait2 = [&](int b, int c) { wait(b + (c & 1), static_cast<uint32_t>((c >> 1) & 1)); };
+    auto publish_state = [&]() {  // S as the A operands of (C S)^T
+      const uint32_t dst = tl + TM_SB + kCols / 2 * cq;
+#pragma unroll
+      for (int part = 0; part < kCols / 16; ++part) {
+        uint32_t w[8], wl[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split(make_float2(s[16 * part + 2 * i], s[16 * part + 2 * i + 1]), w[i], wl[i]);
+        tmem_st8u(dst + 8 * part, w);
+        tmem_st8u(dst + 64 + 8 * part, wl);
+      }
+      tmem_wait_st();
+    };
+    if (!STATE_ONLY) {
+      publish_state();
+      signal(B_RDY_S, false);
+    }
     constexpr int kDsBufs = STATE_ONLY ? 2 : 1;
     auto wait_ds = [&](int c) { wait(B_DS + c % kDsBufs, static_cast<uint32_t>((c / kDsBufs) & 1)); };
 
@@ -633,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (term + 1 < kTerms)  // (a product with -1: packed operands have no sign modifier)
-              v[k][e] = __ffma2_rn(make_float2(bf16_lo(b[k][e]), bf16_hi(b[k][e])), make_float2(-1.f, -1.f), v[k][e]);
+              v[k][e] = minus_bf16x2(v[k][e], b[k][e]);
             else
               chk = __fadd2_rn(chk, v[k][e]);  // the last remainders: NaN where x is not finite
 #pragma unroll
@@ -677,12 +688,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
       reg_fence(v);
       uint32_t m[8], ml[8];
-      // the rounded value, then what it left (as W's terms)
-      auto split = [&](float2 q, uint32_t& hi, uint32_t& lo) {
-        hi = pack_bf16x2(q.x, q.y);
-        const float2 r = __ffma2_rn(make_float2(bf16_lo(hi), bf16_hi(hi)), make_float2(-1.f, -1.f), q);
-        lo = pack_bf16x2(r.x, r.y);
-      };
       if constexpr (kBelow) {
         float u[16];
         load16(tb + G_U + r0, u);
@@ -735,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto make_m = [&](int c, int st, uint32_t st_par) {
       wait(B_X + st, st_par);  // (the tables)
-      if (c > 0) wait2(B_PV, c - 1);  // M is free
+      if (c > 0) wait(B_PV, static_cast<uint32_t>((c - 1) & 1));  // M is free
       wait(B_G, static_cast<uint32_t>(c & 1));
       if (kHeads == 2) {
         if (quarter == 2) {
@@ -763,15 +768,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto outputs = [&](int c, int st) {
       float eg[16], qs[16], pv[16];
       load16(table(st, hh) + G_EG + 16 * cq, eg);
-      if (!has_m || c + 1 == n) wait2(B_PV, c);  // (the others waited for it to write M)
-      if (c + 1 == n) wait2(B_QS, c);  // (before that, the state's update waited for it)
+      if (!has_m || c + 1 == n) wait(B_PV, static_cast<uint32_t>(c & 1));  // (the others waited for it to write M)
+      if (c + 1 == n) wait(B_QS, static_cast<uint32_t>(c & 1));  // (before that, the state's update waited for it)
       const bool bad = *any_bad != 0u;  // (written before this chunk's W was signalled)
-      tmem_ld16(tl + TM_PV + 64 * (c & 1) + 16 * cq, pv);
-      tmem_ld16(tl + TM_QS + 64 * (c & 1) + 16 * cq, qs);
+      tmem_ld16(tl + TM_PV + 64 * hh + 16 * cq, pv);
+      tmem_ld16(tl + TM_QS + 16 * cq, qs);
       tmem_wait_ld();
       reg_fence(pv);
       reg_fence(qs);
-      signal(B_RDY_D + (c & 1), false);
+      signal(B_RDY_D, false);
       float o[16];
 #pragma unroll
       for (int k = 0; k < 16; k += 2) {
@@ -826,6 +831,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld16(tl + TM_DS + 128 * (c % kDsBufs) + 16 * cq, v);
       tmem_wait_ld();
       reg_fence(v);
+      // W^T B has been read: the next may be formed.  (With heads of 64, whose products are longer, while
+      // this warp still publishes: 3 % of the time; with heads of 128 that costs 2 %.)
+      if (!STATE_ONLY && kHeads == 2 && c + 1 < n) signal(B_RDY_S, false);
 #pragma unroll
       for (int i = 0; i < kCols; i += 2) {
         const float2 r = __ffma2_rn(make_float2(dec, dec), make_float2(s[i], s[i + 1]), make_float2(v[i], v[i + 1]));
@@ -833,8 +841,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         s[i + 1] = r.y;
       }
       if (!STATE_ONLY && c + 1 < n) {
-        wait2(B_QS, c);  // the product that reads the last published state is done
+        wait(B_QS, static_cast<uint32_t>(c & 1));  // the product that reads the last published state is done
         publish_state();
+        if (kHeads == 1) signal(B_RDY_S, false);
       }
     };
 
@@ -901,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t idesc_g = idesc_bf16(128, 64, false, false);   // [B; C] B^T
     constexpr uint32_t idesc_ds = idesc_bf16(128, NS, true, true);    // W^T B
     constexpr uint32_t idesc_qs = idesc_bf16(128, 64, false, false);  // S (TMEM) C^T
-    constexpr uint32_t idesc_pv = idesc_bf16(128, 64, true, false);   // X^T M^T
+    constexpr uint32_t idesc_pv = idesc_bf16(128, 64 * kHeads, true, false);   // X^T M^T
     const uint32_t leader = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);  // (uniform)
     const uint32_t sb16 = sb >> 4;
@@ -934,36 +943,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sdesc_sw128_f(bc + ks * 128, 16384, 1024), idesc_ds, part > 0 || ks > 0);
       commit_by(leader, &bars[B_DS + (STATE_ONLY ? c & 1 : 0)]);
     };
-    auto mma_pv = [&](int c, int xst) {
-      const uint32_t xo = L::OFF_X + xst * L::kX;
+    auto mma_pv = [&](int xst) {
 #pragma unroll
-      for (int head = 0; head < kHeads; ++head)
+      for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          // rows 0-63 and 64-127 of X^T are two blocks of 64; with two heads, the block of the
-          // other head is 2 KiB of zeros, so that each head's M meets its own x only
-          uint32_t start = xo + ks * 2048, lbo = 8192;
-          if (kHeads == 2 && head == 0) lbo = L::OFF_Z1 - start;
-          if (kHeads == 2 && head == 1) {
-            lbo = start + 8192 - L::OFF_Z0;
-            start = L::OFF_Z0;
-          }
-          const uint64_t a = sdesc_sw128_f(sb16 + start / 16, lbo, 1024);
-#pragma unroll
-          for (int term = 0; term < kMTerms; ++term)
-            mma_ss_by(leader, tm + TM_PV + 64 * (c & 1), a,
-                      sdesc_sw128_f(sb16 + (L::OFF_M + term * L::kM + head * 8192 + ks * 32) / 16, 16, 1024), idesc_pv,
-                      head > 0 || ks > 0 || term > 0);
-        }
-      commit_by(leader, &bars[B_PV + (c & 1)]);
+        for (int term = 0; term < kMTerms; ++term)
+          mma_ss_by(leader, tm + TM_PV, sdesc_sw128_f(sb16 + (L::OFF_X + ks * 2048) / 16 + xst * (L::kX / 16), 8192, 1024),
+                    sdesc_sw128_f(sb16 + (L::OFF_M + term * L::kM + ks * 32) / 16, 16, 1024), idesc_pv, ks > 0 || term > 0);
+      commit_by(leader, &bars[B_PV]);
     };
-    auto mma_qs = [&](int c, int bst) {
+    auto mma_qs = [&](int bst) {
       const uint32_t bc = sb16 + kBc16 + bst * kBcSize16;
 #pragma unroll
       for (int ks = 0; ks < NS / 16; ++ks)
-        mma_ts_by(leader, tm + TM_QS + 64 * (c & 1), tm + TM_SB + 8 * ks,
-                  sdesc_sw128_f(bc + ((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) / 16, 16, 1024), idesc_qs, ks > 0);
-      commit_by(leader, &bars[B_QS + (c & 1)]);
+#pragma unroll
+        for (int term = 0; term < 2; ++term)
+          mma_ts_by(leader, tm + TM_QS, tm + TM_SB + 64 * term + 8 * ks,
+                    sdesc_sw128_f(bc + ((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) / 16, 16, 1024), idesc_qs, ks > 0 || term > 0);
+      commit_by(leader, &bars[B_QS]);
     };
     bool ok = STATE_ONLY || mma_g(0, 0);
     // stages of chunk c + 1 (of B and C, of x) and of chunk c + 2 (of B and C, with its parity)
@@ -979,18 +976,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_ds(c + 1, b1);
         commit_by(leader, &bars[B_EMPTY + b1]);
       } else {
-        // the outputs of chunk c - 1 have read the buffers that chunk c + 1 takes
-        if (c >= 1 && !(ok = wait(B_RDY_D + static_cast<int>(next), static_cast<uint32_t>(((c - 1) >> 1) & 1)))) break;
         if (!(ok = wait(B_RDY_M, next))) break;
-        // (with two stages of B and C, chunk c + 2's are just being loaded)
-        if (kBcStages == 3 && c + 2 < n && !(ok = mma_g(b2, par2))) break;
+        // (G right behind M: the warps that form M wait for it.  After C S it cost 3 %.)
+        if (c + 2 < n && !(ok = mma_g(b2, par2))) break;
         if (!(ok = wait(B_RDY_W, next))) break;
-        mma_pv(c + 1, x1);
         if (!(ok = wait(B_RDY_S, next))) break;  // the update of chunk c has read W^T B
         mma_ds(c + 1, b1);
-        mma_qs(c + 1, b1);
+        // the state that C reads is published and the outputs of chunk c have read their accumulators
+        if (c >= 0 && !(ok = wait(B_RDY_D, static_cast<uint32_t>(c & 1)))) break;
+        mma_pv(x1);
+        mma_qs(b1);
         commit_by(leader, &bars[B_EMPTY + b1]);
-        if (kBcStages == 2 && c + 2 < n && !(ok = mma_g(b2, par2))) break;
       }
       b1 = b2;
       par1 = par2;
@@ -1054,9 +1050,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             make_float2(dt[0] * ex2_ftz(first - gt[0]), dt[1] * ex2_ftz(first - gt[1]));
         *reinterpret_cast<float2*>(tb + G_W + 2 * lane) = make_float2(dt[0] * ex2_ftz(rest[0]), dt[1] * ex2_ftz(rest[1]));
         const float nan = __int_as_float(0x7fc00000);
-        const int fy = skip_ok ? fb : 0;  // first output that is not finite
         *reinterpret_cast<float2*>(tb + G_EG + 2 * lane) =
-            make_float2(2 * lane >= fy ? nan : ex2_ftz(gt[0]), 2 * lane + 1 >= fy ? nan : ex2_ftz(gt[1]));
+            make_float2(2 * lane >= fb ? nan : ex2_ftz(gt[0]), 2 * lane + 1 >= fb ? nan : ex2_ftz(gt[1]));
         if (lane == 0) {
           decs[buf * 2 + gh] = fb < 64 ? nan : ex2_ftz(g63);
           steep[buf * 2 + gh] = (far & 1u) | (far >> 7 & 2u) | (far >> 14 & 4u) | (far >> 21 & 8u);

@@ -75,10 +75,31 @@ def test_outputs_within_a_chunk_are_rounded_once(H, P, G, Ns):
     rounded_once(out, y, out_slack(ya, 64))
 
 
+@pytest.mark.parametrize("H,P,G,Ns,lens,state", [
+    (3, 64, 1, 128, [200, 65, 130], True), (2, 128, 1, 128, [129, 0, 400], True), (4, 64, 2, 64, [700], True),
+    (2, 128, 2, 64, [64, 100], True),
+    (6, 128, 2, 128, [150, 64], False),            # three heads of 128 a group
+    (2, 64, 1, 128, [1900], True), (2, 128, 2, 64, [3300, 5], False)])  # in pieces
+def test_outputs_and_states_of_long_sequences(H, P, G, Ns, lens, state):
+    """Outputs rounded once.  States as fp32 sums give them, by their norm too: three bf16 terms of W leave 2^-24 of a
+    term; each token's decay and product are off by 8 2^-24 at most, and such errors, of either sign, come to less
+    than a millionth of the whole (two terms of W left 2.6e-6)."""
+    m = make((sum(lens),), H, P, G, Ns, seed=24 + H)
+    st = torch.randn(len(lens), H, P, Ns, device="cuda") if state else None
+    out, new = run(m, lens, st)
+    y, ya, S, _ = reference(m, lens, st)
+    rounded_once(out, y, out_slack(ya, max(lens)))
+    own = (y.to(torch.bfloat16).double() - y).norm()
+    assert (L.d(out) - y).norm() <= 1.02 * own
+    for i, n in enumerate(lens):
+        if n or st is not None:
+            assert (L.d(new[i]) - S[i]).norm() <= 1e-6 * S[i].norm()
+
+
 @pytest.mark.parametrize("value", ["nan", "inf", "-inf", "3e38"])
 @pytest.mark.parametrize("P,lens", [(64, [100, 70]), (128, [100, 70]), (64, [1900])])
 def test_a_skip_that_is_not_finite_stays_in_its_head(P, lens, value):
-    """Two heads of 64 share a tile's products.  (3e38: finite, but an operand that large is taken as if it were not.)"""
+    """Two heads of 64 share a tile's products."""
     m = make((sum(lens),), 4, P, 2, 128, seed=22)
     want, want_s = run(m, lens)
     for head in (1, 2):
@@ -87,7 +108,26 @@ def test_a_skip_that_is_not_finite_stays_in_its_head(P, lens, value):
         got, got_s = run(bad, lens)
         rest = [h for h in range(4) if h != head]
         assert torch.equal(got[:, rest], want[:, rest]) and torch.equal(got_s, want_s)
-        assert not got[:, head].isfinite().any()
+        if value == "3e38":  # (finite, and so are its products with x below 1)
+            y, ya, _, _ = reference(bad, lens)
+            small = bad["x"][:, head].abs().cpu() < 1
+            rounded_once(got[:, head][small.cuda()], y[:, head][small], out_slack(ya[:, head][small], max(lens)))
+        else:
+            assert not got[:, head].isfinite().any()
+
+
+@pytest.mark.parametrize("lens", [[100, 70], [1900]])
+def test_a_step_that_overflows_stays_in_its_head(lens):
+    """A step of 3e38 at one token: the weights of its head within the chunk overflow."""
+    m = make((sum(lens),), 4, 64, 2, 128, seed=25)
+    want, want_s = run(m, lens)
+    for head in (1, 2):
+        bad = dict(m, a=m["a"].clone())
+        bad["a"][40, head] = 3e38
+        got, got_s = run(bad, lens)
+        rest = [h for h in range(4) if h != head]
+        assert torch.equal(got[:, rest], want[:, rest]) and torch.equal(got_s[:, rest], want_s[:, rest])
+        assert torch.equal(got[:40], want[:40]) and torch.equal(got[lens[0]:], want[lens[0]:])
 
 
 @pytest.mark.parametrize("what", ["x nan", "x inf", "a nan", "B nan", "C inf"])
