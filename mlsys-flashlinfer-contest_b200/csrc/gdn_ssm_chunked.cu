@@ -555,11 +555,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < pc.index; ++j) {  // through the pieces before this one
         // (the bound holds for any cu_seqlens)
         const int64_t u = min(static_cast<int64_t>(pc.before) + j, p.inner - 1) * p.tiles + tile;
-        const float dec = p.ws_dec[2 * u + hh];
+        // (coherent loads, past L1: this grid is resident while the first launch still writes the
+        // pieces' states, so the read-only path, which wants memory that nobody writes for the whole life of the
+        // grid, may not be taken)
+        const float dec = __ldcg(p.ws_dec + 2 * u + hh);
         const float4* F = reinterpret_cast<const float4*>(p.ws) + u * (kRows * NS / 4) + tid;
 #pragma unroll
         for (int i = 0; i < kCols / 4; ++i) {
-          const float4 v = __ldg(F + i * kComputeThreads);
+          const float4 v = __ldcg(F + i * kComputeThreads);
           s[4 * i] = fmaf(dec, s[4 * i], v.x);
           s[4 * i + 1] = fmaf(dec, s[4 * i + 1], v.y);
           s[4 * i + 2] = fmaf(dec, s[4 * i + 2], v.z);
