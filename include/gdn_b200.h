@@ -399,7 +399,7 @@ int gdn_ssm_pool(const void *x, const void *B, const void *C, const float *A_log
  *             (NULL without residual; may be residual itself when that is contiguous)
  *   output    [rows, dim] of `dtype`, or with `scale` e4m3 (1 byte): y / scale with
  *   scale     [rows] (group_size 0) or [rows, dim / 128] (group_size 128) fp32:
- *             max |y| of the row or group / 448 (1 where that maximum is below 2^-100)
+ *             max |y| of the row or group / 448 (1 where that is 0)
  * A 16-bit output or residual_out may be one of the inputs that is contiguous, as a whole;
  * no other overlap is allowed.  Squares are summed in fp32: above 1e18 they overflow.
  * y is fp32 up to the output's one rounding.  dim is a multiple of 8 (of 128 with
