@@ -322,8 +322,8 @@ enum gdn_dtype { GDN_BF16 = 0, GDN_F16 = 1 };
  * of 8 and every buffer 16-byte aligned.  Sums are fp32, rounded once.  A sequence of
  * length 0 keeps its state.  Rows of no sequence (before cu_seqlens[0] or from
  * cu_seqlens[N] on) are left as they were.  new_state and the outputs may not overlap
- * x (from its first row to its last), state, weight, bias or one another.  silu is
- * -0 for sums below -41.5, NaN for -inf.  cu_seqlens is read only on the device, clamped to [0, T].
+ * x (from its first row to its last), state, weight, bias or one another.  silu of -inf
+ * is NaN.  cu_seqlens is read only on the device, clamped to [0, T].
  */
 int gdn_conv(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
              const void *state, const int64_t *cu_seqlens, void *const *outputs,

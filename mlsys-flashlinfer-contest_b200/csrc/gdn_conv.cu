@@ -130,16 +130,20 @@ __device__ __forceinline__ void load_weights(const ConvParams& p, int64_t c0, fl
   }
 }
 
-// silu of two values with one reciprocal: 1 / (a b) gives both, a = 1 + 2^(-x log2 e).  The
-// exponents are held below 2^60, so that the product stays finite; where one would exceed that,
-// x < -41.5, the sigmoid is 0 instead of less than 2^-59 (x 2^-60 would be 1e20 for the type's
-// lowest value); -inf gives NaN, as in the formula.  fminf also keeps a NaN to its own result.  MUFU
-// operations bound the convolution next to HBM: three for two values instead of four.
+// silu x = x t^2 / (1 + t^2) with t = e^(x/2), for two values with one reciprocal: 1 / (a b) gives both,
+// a = 1 + t^2.  MUFU operations bound the convolution next to HBM: three for two values instead of four.
+// The exponents of t are held at 30, so that the product stays finite (the sigmoid is 1 there, to 2^-60);
+// below, x t and t reach as far down as the type does, with neither clamp nor selection.  NaN and
+// -inf give NaN, as in the formula, and fminf keeps a NaN to its own result.  (In scalar operations
+// 3-5 % slower for prompts.)
 __device__ __forceinline__ void silu2(float& x, float& y) {
-  const float a = 1.0f + ex2_ftz(fminf(-x * kLog2e, 60.f)), b = 1.0f + ex2_ftz(fminf(-y * kLog2e, 60.f));
-  const float r = rcp_approx(a * b);
-  x *= x < -41.5f ? 0.f : r * b;
-  y *= y < -41.5f ? 0.f : r * a;
+  const float2 z = __fmul2_rn(make_float2(x, y), make_float2(0.5f * kLog2e, 0.5f * kLog2e));
+  const float2 t = make_float2(ex2_ftz(fminf(z.x, 30.f)), ex2_ftz(fminf(z.y, 30.f)));
+  const float2 a = __ffma2_rn(t, t, make_float2(1.f, 1.f));
+  const float r = rcp_approx(a.x * a.y);
+  const float2 v = __fmul2_rn(__fmul2_rn(make_float2(x, y), t), __fmul2_rn(t, __fmul2_rn(make_float2(r, r), make_float2(a.y, a.x))));
+  x = v.x;
+  y = v.y;
 }
 
 // One output row from the window (W - 1 earlier rows, oldest first) and the current row.

@@ -65,10 +65,9 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
 }
 
 // x sigmoid(x) from the hardware 2^x and reciprocal (each within 2 ulp of fp32,
-// far below the 16-bit output's step).  For x below -88, 2^(-x log2 e) is +inf and
-// its reciprocal 0: the result is -0, as in exact arithmetic rounded to 16 bits;
-// -inf gives -inf * 0 = NaN and is mapped to the limit 0 nowhere: like the formula
-// evaluated in fp32, it stays NaN.
+// far below the 16-bit output's step).  For x below -87 the reciprocal of 1 + e^-x is
+// below fp32's normal range and the result -0 (less than 2^-119 in exact arithmetic);
+// -inf gives -inf * 0 = NaN, like the formula evaluated in fp32.
 __device__ __forceinline__ float silu(float x) { return x * sigmoid_fast(x); }
 
 }  // namespace gdn
