@@ -1182,8 +1182,13 @@ constexpr double kStateChunk = 0.4, kCta = 3.0, kJoin = 0.3, kLaunch = 1.5;
 
 // Only the mean length is known here (the lengths lie on the device): the piece length is the
 // one that is best for sequences of that length.  Calls that fill the SMs with whole sequences
-// are cut too, but only sequences of twice the work of an SM: one long sequence among short
-// ones would run on alone for most of the call.
+// are cut too, but only sequences of twice the work of an SM, which would run on alone for most
+// of the call; where there are none, the first launch and the search cost ~4 us.  That is done where a
+// sequence of that length is either likely (twice the mean) or a small part of the call (a quarter), so that
+// cutting it gains much.  Measured, whole | cut, 64 heads of 64 unless said: 4 sequences, 65536 tokens,
+// even 699 | 701 us, ragged 1272 | 1131, half the tokens in one 1634 | 1125; 128 sequences, 16384
+// tokens, 32 heads, even 155 | 156, half in one 380 | 228.  Not done: 16 sequences, 7648 tokens, even
+// 111 | 115, ragged 120 | 123, half in one 190 | 147.
 Cut choose_cut(int64_t T, int64_t N, int64_t tiles, int sms) {
   const int64_t chunks = std::max<int64_t>(1, (T + N * kChunk - 1) / (N * kChunk));  // of a mean sequence
   auto waves = [&](int64_t ctas) { return static_cast<double>((ctas + sms - 1) / sms); };
@@ -1202,7 +1207,7 @@ Cut choose_cut(int64_t T, int64_t N, int64_t tiles, int sms) {
   }
   const int64_t all = T / kChunk, share = (all * tiles + sms - 1) / sms;  // chunks of an SM, were they spread evenly
   const int64_t longest = std::max(2 * share, chunks + 1);
-  if (best.seg == 0 && all >= 64 && 2 * longest <= all) best.seg = longest;
+  if (best.seg == 0 && all >= 64 && 2 * longest <= all && (longest <= 2 * chunks || 4 * longest <= all)) best.seg = longest;
   if (best.seg) {
     best.seg *= kChunk;
     best.slots = N + T / best.seg;  // the pieces of N sequences of T tokens are at most this many
