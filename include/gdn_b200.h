@@ -356,7 +356,7 @@ int gdn_conv_pool(const void *x, int64_t x_batch_stride, int64_t x_row_stride, c
  *   A_log, dt_bias [H] fp32                D        [H] fp32 or NULL (no skip term)
  *   cu_seqlens [N+1] int64, device         output   [T, H, P] bf16
  *   new_state [N, H, P, Ns] fp32
- * output and new_state may not overlap an input or one another.
+ * output, new_state and workspace may not overlap an input or one another.
  * P (head_dim) and Ns (state_dim) are 64 or 128; num_heads is a multiple of num_groups.
  * The state is in the k-last layout of gdn_prefill.  A sequence of length 0 keeps its
  * state.  Rows of no sequence are left as they were.  Buffers need 16-byte alignment.
@@ -400,8 +400,8 @@ int gdn_ssm_pool(const void *x, const void *B, const void *C, const float *A_log
  *   output    [rows, dim] of `dtype`, or with `scale` e4m3 (1 byte): y / scale with
  *   scale     [rows] (group_size 0) or [rows, dim / 128] (group_size 128) fp32:
  *             max |y| of the row or group / 448 (1 where that is 0)
- * A 16-bit output or residual_out may be one of the inputs that is contiguous, as a whole;
- * no other overlap is allowed.  Squares are summed in fp32: above 1e18 they overflow.
+ * A 16-bit output or residual_out may be one of x, residual and gate that is contiguous, as a
+ * whole; no other overlap is allowed.  Squares are summed in fp32: above 1e18 they overflow.
  * y is fp32 up to the output's one rounding.  dim is a multiple of 8 (of 128 with
  * group_size 128) up to 16384; strides are multiples of 8, buffers 16-byte aligned.
  */

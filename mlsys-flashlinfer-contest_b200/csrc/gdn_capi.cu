@@ -562,13 +562,14 @@ static bool ssm_recurrent(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P)
 
 // The scan's outputs against its inputs, `rows` tokens and states of `bytes` bytes.  (A call in two
 // launches reads x and a in the first while the second writes.)
-static bool ssm_overlap(const gdn::SsmArgs& p, int64_t rows, const void* states, const void* new_states, size_t bytes) {
+static bool ssm_overlap(const gdn::SsmArgs& p, int64_t rows, const void* states, const void* new_states, size_t bytes,
+                        Range workspace) {
   const size_t x = static_cast<size_t>(rows) * p.H * p.P * 2, b = static_cast<size_t>(rows) * p.G * p.Ns * 2,
                heads = static_cast<size_t>(p.H) * 4;
-  const Range w[2] = {{p.out, x}, {new_states, bytes}};
+  const Range w[3] = {{p.out, x}, {new_states, bytes}, workspace};
   const Range r[8] = {{p.x, x}, {p.B, b}, {p.C, b}, {p.a, static_cast<size_t>(rows) * p.H * 2}, {states, bytes},
                       {p.A_log, heads}, {p.dt_bias, heads}, {p.D, heads}};
-  return any_overlap(w, 2, r, 8);
+  return any_overlap(w, 3, r, 8);
 }
 
 size_t gdn_ssm_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t G, int64_t P, int64_t Ns) {
@@ -599,7 +600,7 @@ int gdn_ssm(const void* x, const void* B, const void* C, const float* state, con
   p.x = x, p.B = B, p.C = C, p.state = state, p.A_log = A_log, p.a = a, p.dt_bias = dt_bias, p.D = D;
   p.cu_seqlens = cu_seqlens, p.out = output, p.new_state = new_state;
   p.T = T, p.N = N, p.H = H, p.G = G, p.P = P, p.Ns = Ns;
-  if (ssm_overlap(p, T, state, new_state, bytes)) return fail(GDN_ERR_VALUE, "an output overlaps another tensor");
+  if (ssm_overlap(p, T, state, new_state, bytes, {workspace, need})) return fail(GDN_ERR_VALUE, "an output overlaps another tensor");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (ssm_recurrent(T, N, H, G, P)) return cuda_status(gdn::launch_ssm_recurrent(p, st), "gdn_ssm launch");
   return cuda_status(gdn::launch_ssm_chunked(p, need ? workspace : nullptr, sm_count(), st), "gdn_ssm launch");
@@ -629,7 +630,7 @@ int gdn_ssm_pool(const void* x, const void* B, const void* C, const float* A_log
   p.state_bf16 = state_dtype == GDN_STATE_BF16;
   p.no_state_update = (flags & GDN_POOL_NO_STATE_UPDATE) != 0;
   if (ssm_overlap(p, batch * T, nullptr, state_pool,
-                  static_cast<size_t>(pool_size) * H * P * Ns * (p.state_bf16 ? 2 : 4)))
+                  static_cast<size_t>(pool_size) * H * P * Ns * (p.state_bf16 ? 2 : 4), {nullptr, 0}))
     return fail(GDN_ERR_VALUE, "an output overlaps another tensor");
   return cuda_status(gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream)), "gdn_ssm_pool launch");
 }
@@ -673,6 +674,14 @@ int gdn_rms_norm(const void* x, int64_t x_stride, const void* weight, const void
       return fail(GDN_ERR_VALUE, "an output overlaps an input without being the same buffer");
   }
   if (overlap(output, out_bytes, residual_out, flat)) return fail(GDN_ERR_VALUE, "output overlaps residual_out");
+  // the scales and the weight share nothing
+  const Range written[3] = {{output, out_bytes}, {residual_out, flat},
+                            {scale, static_cast<size_t>(rows) * (group ? D / group : 1) * 4}};
+  for (int i = 0; i < 3; ++i)
+    if (overlap(weight, static_cast<size_t>(D) * 2, written[i].p, written[i].bytes) ||
+        overlap(written[2].p, written[2].bytes, in[i].p, in[i].bytes) ||
+        (i < 2 && overlap(written[2].p, written[2].bytes, written[i].p, written[i].bytes)))
+      return fail(GDN_ERR_VALUE, "weight or scale overlaps another tensor");
   const gdn::NormArgs a{x, weight, residual, gate, output, scale, residual_out, x_stride, residual_stride,
                         gate_stride, rows, D, group, eps, dtype == GDN_F16,
                         (flags & GDN_NORM_GATE_FIRST) != 0};
