@@ -33,7 +33,7 @@ def test_norm(kw):
     assert rc == N.GDN_ERR_VALUE and "overlaps" in msg
 
 
-@pytest.mark.parametrize("ws", [1 * MB + 256, 6 * MB, 6 * MB + (1 << 19) - 256, 8 * MB - 256])
+@pytest.mark.parametrize("ws", [1 * MB + 256, 6 * MB, 6 * MB + 2000 * 256 - 256, 8 * MB - 256])
 def test_scan_workspace(ws):
     """A call in two launches: its pieces' states over x, the output, the new states."""
     T, n, H, G, Pd, Ns = 2000, 1, 2, 1, 64, 128
