@@ -39,6 +39,12 @@ NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3"
                      "--expt-relaxed-constexpr", "-I", str(CSRC), "-I", str(REPO / "include")]
 
 
+# The extension modules take the C++ library of the process.  A compiler that only has the archive links a
+# second one into them, whose streams and locales are mixed with the first's: inserting a number into the
+# stream of an error message then crashes.  Named first, the shared one leaves the archive nothing to add.
+CXX_RUNTIME = ["-l:libstdc++.so.6"]
+
+
 def nvcc() -> str:
     for cand in (os.environ.get("NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
         if cand and Path(cand).exists():
@@ -103,7 +109,7 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
            "-DTORCH_EXTENSION_NAME=_gdn_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
            *[f"-I{p}" for p in incs], str(src), "-o", str(tmp),
            f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
-           f"-L{LIB.parent}", "-lgdn_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
+           f"-L{LIB.parent}", "-lgdn_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}", *CXX_RUNTIME]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -130,7 +136,7 @@ def build_tvm_ffi(force: bool = False, verbose: bool = False) -> Path:
            *[f"-I{p}" for p in incs], str(src), "-o", str(tmp),
            f"-L{ffi_lib.parent}", "-ltvm_ffi", f"-L{cuda / 'lib64'}", "-lcudart",
            f"-L{LIB.parent}", "-lgdn_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{ffi_lib.parent}",
-           f"-Wl,-rpath,{cuda / 'lib64'}"]
+           f"-Wl,-rpath,{cuda / 'lib64'}", *CXX_RUNTIME]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -26,9 +26,7 @@ void cuda_contig(const at::Tensor& t, const char* name) {
 }
 
 void rank(const at::Tensor& t, const char* name, int64_t d) {
-  // (numbers go into messages through std::to_string: inserting them into the message's
-  // stream crashes in a process that has loaded the CUDA libraries)
-  TORCH_CHECK_VALUE(t.dim() == d, name, " must be a ", std::to_string(d), "D tensor");
+  TORCH_CHECK_VALUE(t.dim() == d, name, " must be a ", d, "D tensor");
 }
 
 void dtype(const at::Tensor& t, const char* name, at::ScalarType s) {
