@@ -49,6 +49,7 @@
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 #include "gdn_sm100.cuh"
+#include "gdn_tmap.h"
 
 namespace gdn {
 
@@ -597,24 +598,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      ptr = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }();
-  return fn;
-}
-
 // [d2][d1][128] bf16 viewed with box {64, b1, b2}, 128-byte swizzle: the pool as
 // [P*Hv tiles][128 rows][128] (box = one 64-column block of a tile) and q/k/v as
 // [B*T][heads][128] (box = T token rows of one head, 64 columns).
 cudaError_t encode_rows(CUtensorMap* m, const void* base, uint64_t d1, uint64_t d2, uint32_t b1,
                         uint32_t b2) {
-  auto fn = encoder();
+  auto fn = tmap_encoder();
   if (!fn) return cudaErrorNotSupported;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(kHead), d1, d2};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(kHead) * 2, static_cast<cuuint64_t>(d1) * kHead * 2};
@@ -628,7 +617,7 @@ cudaError_t encode_rows(CUtensorMap* m, const void* base, uint64_t d1, uint64_t 
 
 // gate inputs [B*T][Hv] bf16, box = T rows of 8 heads (16 bytes), no swizzle
 cudaError_t encode_gates(CUtensorMap* m, const void* base, uint64_t Hv, uint64_t rows, uint32_t T) {
-  auto fn = encoder();
+  auto fn = tmap_encoder();
   if (!fn) return cudaErrorNotSupported;
   cuuint64_t dims[2] = {Hv, rows};
   cuuint64_t strides[1] = {Hv * 2};

@@ -45,6 +45,7 @@
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 #include "gdn_sm100.cuh"
+#include "gdn_tmap.h"
 
 namespace gdn {
 
@@ -1299,22 +1300,9 @@ __global__ void gdn_wait_probe_kernel(uint64_t timeout_ns, uint32_t* result) {
 }
 
 // ---- host side ---------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      ptr = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }();
-  return fn;
-}
-
 // [T, heads, 128] bf16, box = 64 tokens x 1 head x 64 dims, 128-byte swizzle.
 cudaError_t encode_head_map(CUtensorMap* m, const void* base, int64_t heads, int64_t T) {
-  auto fn = encode_fn();
+  auto fn = tmap_encoder();
   if (!fn) return cudaErrorNotSupported;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(kHead), static_cast<cuuint64_t>(heads),
                         static_cast<cuuint64_t>(T)};
@@ -1331,7 +1319,7 @@ cudaError_t encode_head_map(CUtensorMap* m, const void* base, int64_t heads, int
 // The initial state [rows = N Hv 128][128] fp32, box 32 columns x 128 rows (one
 // column quarter of a tile), 128-byte swizzle.
 cudaError_t encode_state_map(CUtensorMap* m, const void* base, int64_t rows) {
-  auto fn = encode_fn();
+  auto fn = tmap_encoder();
   if (!fn) return cudaErrorNotSupported;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(kHead), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(kHead) * 4};
@@ -1343,31 +1331,11 @@ cudaError_t encode_state_map(CUtensorMap* m, const void* base, int64_t rows) {
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// Encoding a tensor map costs about a microsecond of host time and a call needs
-// four or five; a small per-thread cache of encoded maps, keyed by what the
-// encoding depends on (base address, heads, T; heads = 0 marks a state map of T
-// rows), skips it when a caller reuses its buffers (a serving loop, or the caching
-// allocator handing back a block).
+// (heads = 0: a state map of T rows)
 cudaError_t make_head_map(CUtensorMap* m, const void* base, int64_t heads, int64_t T) {
-  struct Entry {
-    const void* base;
-    int64_t heads, T;
-    CUtensorMap map;
-  };
-  constexpr int kEntries = 16;
-  thread_local Entry cache[kEntries];
-  thread_local int used = 0, next = 0;
-  for (int i = 0; i < used; ++i)
-    if (cache[i].base == base && cache[i].heads == heads && cache[i].T == T) {
-      *m = cache[i].map;
-      return cudaSuccess;
-    }
-  const cudaError_t e = heads == 0 ? encode_state_map(m, base, T) : encode_head_map(m, base, heads, T);
-  if (e != cudaSuccess) return e;
-  cache[next] = Entry{base, heads, T, *m};
-  next = (next + 1) % kEntries;
-  if (used < kEntries) ++used;
-  return cudaSuccess;
+  return cached_tmap(m, {base, {heads, T, 0}}, [=](CUtensorMap* map) {
+    return heads == 0 ? encode_state_map(map, base, T) : encode_head_map(map, base, heads, T);
+  });
 }
 
 template <bool DEBUG>

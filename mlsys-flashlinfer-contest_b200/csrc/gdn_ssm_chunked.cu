@@ -60,6 +60,7 @@
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 #include "gdn_sm100.cuh"
+#include "gdn_tmap.h"
 
 namespace gdn {
 
@@ -1115,58 +1116,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---- host side ---------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      ptr = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }();
-  return fn;
+// [T, heads, inner] bf16, box = 64 tokens x 1 head x 64 values, or (heads = 0) [T, inner] fp32,
+// box = 64 rows x 32 values; 128-byte swizzle.
+cudaError_t encode_map(CUtensorMap* m, const void* base, int64_t inner, int64_t heads, int64_t T) {
+  auto fn = tmap_encoder();
+  if (!fn) return cudaErrorNotSupported;
+  const bool tokens = heads != 0;
+  const cuuint64_t n = static_cast<cuuint64_t>(inner), h = static_cast<cuuint64_t>(heads), t = static_cast<cuuint64_t>(T);
+  const cuuint64_t dims[3] = {n, tokens ? h : t, t}, strides[2] = {n * (tokens ? 2 : 4), h * n * 2};
+  const cuuint32_t box[3] = {tokens ? 64u : 32u, tokens ? 1u : 64u, 64}, es[3] = {1, 1, 1};
+  const CUresult r = fn(m, tokens ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, tokens ? 3 : 2,
+                        const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// [T, heads, inner] bf16, box = 64 tokens x 1 head x 64 values, or (heads = 0) [T, inner] fp32,
-// box = 64 rows x 32 values; 128-byte swizzle.  A small cache per thread spares a caller that
-// reuses its buffers the ~1 us of an encoding.
 cudaError_t make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t heads, int64_t T) {
-  struct Entry {
-    const void* base;
-    int64_t inner, heads, T;
-    CUtensorMap map;
-  };
-  constexpr int kEntries = 16;
-  thread_local Entry cache[kEntries];
-  thread_local int used = 0, next = 0;
-  for (int i = 0; i < used; ++i)
-    if (cache[i].base == base && cache[i].inner == inner && cache[i].heads == heads && cache[i].T == T) {
-      *m = cache[i].map;
-      return cudaSuccess;
-    }
-  auto fn = encode_fn();
-  if (!fn) return cudaErrorNotSupported;
-  const cuuint64_t n = static_cast<cuuint64_t>(inner), h = static_cast<cuuint64_t>(heads), t = static_cast<cuuint64_t>(T);
-  const cuuint32_t es[3] = {1, 1, 1};
-  CUresult r;
-  if (heads) {
-    const cuuint64_t dims[3] = {n, h, t}, strides[2] = {n * 2, h * n * 2};
-    const cuuint32_t box[3] = {64, 1, 64};
-    r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  } else {
-    const cuuint64_t dims[2] = {n, t}, strides[1] = {n * 4};
-    const cuuint32_t box[2] = {32, 64};
-    r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, es,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  }
-  if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
-  cache[next] = Entry{base, inner, heads, T, *m};
-  next = (next + 1) % kEntries;
-  if (used < kEntries) ++used;
-  return cudaSuccess;
+  return cached_tmap(m, {base, {inner, heads, T}},
+                     [=](CUtensorMap* map) { return encode_map(map, base, inner, heads, T); });
 }
 
 int64_t head_tiles(int64_t H, int64_t G, int64_t P) { return G * ((H / G * P + kRows - 1) / kRows); }
