@@ -95,7 +95,8 @@ constexpr int G_DT = 128;   // dt (0 past the end)
 constexpr int G_U = 192;    // dt 2^(gamma of the last token of t's 16 - gamma_t)
 constexpr int G_W = 256;    // dt 2^(gamma_63 - gamma_t)
 constexpr int G_EG = 320;   // 2^gamma_t
-constexpr int kGateFloats = 384;
+constexpr int G_LOW = 384;  // what gamma's rounding to fp32 left of it
+constexpr int kGateFloats = 448;
 
 // ---- shared memory (offsets from a 1024-aligned base) ------------------------
 template <int P, int NS>
@@ -685,7 +686,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr bool kBelow = decltype(below)::value;  // the block lies below the diagonal
       const int r0 = 16 * cb;
       const float* tb = table(st, head);
-      const float r = ex2_ftz(tb[G_GAM + mi] - tb[G_GAM + r0 + (kBelow ? 15 : 0)]);
+      const int ref = r0 + (kBelow ? 15 : 0);
+      const float r = ex2_ftz((tb[G_GAM + mi] - tb[G_GAM + ref]) + (tb[G_LOW + mi] - tb[G_LOW + ref]));
       const bool far = !kBelow && (steep[st * 2 + head] >> cb & 1u);
       float v[16];
       tmem_ld16(tl + TM_G + r0, v);
@@ -714,12 +716,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             q[k] = __ffma2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
                               make_float2(r, r), make_float2(skip[2 * k], skip[2 * k + 1]));
         } else {
-          const float gi = tb[G_GAM + mi];
+          const float gi = tb[G_GAM + mi], li = tb[G_LOW + mi];
+          auto decay = [&](int j) { return ex2_ftz(fminf((gi - tb[G_GAM + j]) + (li - tb[G_LOW + j]), 0.f)) * tb[G_DT + j]; };
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int j = r0 + 2 * k;
-            q[k].x = fmaf(v[2 * k], ex2_ftz(fminf(gi - tb[G_GAM + j], 0.f)) * tb[G_DT + j], skip[2 * k]);
-            q[k].y = fmaf(v[2 * k + 1], ex2_ftz(fminf(gi - tb[G_GAM + j + 1], 0.f)) * tb[G_DT + j + 1], skip[2 * k + 1]);
+            q[k].x = fmaf(v[2 * k], decay(j), skip[2 * k]);
+            q[k].y = fmaf(v[2 * k + 1], decay(j + 1), skip[2 * k + 1]);
           }
         }
         const uint4* mask = reinterpret_cast<const uint4*>(smem + L::OFF_MASK + md * L::kMaskPitch);
@@ -1024,41 +1027,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (c + 1 < n) load_gates(c + 1);
         const unsigned bad0 = __ballot_sync(0xffffffffu, !ok[0]), bad1 = __ballot_sync(0xffffffffu, !ok[1]);
         const int fb = min(bad0 ? 2 * (__ffs(bad0) - 1) : 64, bad1 ? 2 * (__ffs(bad1) - 1) + 1 : 64);
-        const float pair = lg[0] + lg[1];
-        float incl = pair, suf = pair;
+        // (formed before the tables' places are free)
+        float high[2], low[2], u[2], v[2], w[2], eg[2], total;
+        unsigned far = 0;
+        if constexpr (STATE_ONLY) {  // only W and the chunk's decay: gamma_63 - gamma_t, as sums of their own terms
+          float suf = lg[0] + lg[1];
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const float y = __shfl_up_sync(0xffffffffu, incl, d);
-          const float z = __shfl_down_sync(0xffffffffu, suf, d);
-          if (lane >= d) incl += y;
-          if (lane + d < 32) suf += z;
+          for (int d = 1; d < 32; d <<= 1) {
+            const float z = __shfl_down_sync(0xffffffffu, suf, d);
+            if (lane + d < 32) suf += z;
+          }
+          const float after = __shfl_down_sync(0xffffffffu, suf, 1);
+          const float tail = lane == 31 ? 0.f : after;
+          w[0] = dt[0] * ex2_ftz(tail + lg[1]);
+          w[1] = dt[1] * ex2_ftz(tail);
+          total = suf;
+        } else {
+          // gamma in 64 bits, and its differences: fp32 sums that a strong decay has made large (the
+          // end of a head's memory) would lose the weak ones behind it.  (The fp64 additions are not waited for
+          // here; in the first launch, with a chunk in 1 us, they were: +10 % of a call that is cut.)
+          double incl = static_cast<double>(lg[0]) + lg[1];
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += y;
+          }
+          const double gt[2] = {incl - lg[1], incl};
+          const double first = __shfl_sync(0xffffffffu, gt[0], lane & 24);
+          const double top = __shfl_sync(0xffffffffu, gt[1], lane | 7);
+          const double g63 = __shfl_sync(0xffffffffu, gt[1], 31);
+          far = __ballot_sync(0xffffffffu, first - top > 64.0);
+          auto decay = [](double from, double to) { return ex2_ftz(static_cast<float>(to - from)); };
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            high[e] = static_cast<float>(gt[e]);
+            low[e] = static_cast<float>(gt[e] - high[e]);
+            u[e] = dt[e] * decay(gt[e], top);
+            v[e] = dt[e] * decay(gt[e], first);
+            w[e] = dt[e] * decay(gt[e], g63);
+            eg[e] = 2 * lane + e >= fb ? __int_as_float(0x7fc00000) : ex2_ftz(high[e]);
+          }
+          total = static_cast<float>(g63);
         }
-        const float gt[2] = {incl - lg[1], incl};
-        // gamma_63 - gamma_t as a sum of its own terms (a difference of two long sums would lose
-        // the weights' precision where the decay is strong)
-        const float after = __shfl_down_sync(0xffffffffu, suf, 1);
-        const float tail = lane == 31 ? 0.f : after;
-        const float rest[2] = {tail + lg[1], tail};
-        const float first = __shfl_sync(0xffffffffu, gt[0], lane & 24);
-        const float top = __shfl_sync(0xffffffffu, gt[1], lane | 7);
-        const float g63 = __shfl_sync(0xffffffffu, gt[1], 31);
-        const unsigned far = __ballot_sync(0xffffffffu, first - top > 64.f);
         if (c >= kStages && !__all_sync(0xffffffffu, mbar_test(&bars[B_DONE + buf], par ^ 1u)))
           failed = !__all_sync(0xffffffffu, wait_long(&bars[B_DONE + buf], par ^ 1u));
         if (failed) break;
         float* tb = gates + (buf * 2 + gh) * kGateFloats;
-        *reinterpret_cast<float2*>(tb + G_GAM + 2 * lane) = make_float2(gt[0], gt[1]);
-        *reinterpret_cast<float2*>(tb + G_DT + 2 * lane) = make_float2(dt[0], dt[1]);
-        *reinterpret_cast<float2*>(tb + G_U + 2 * lane) = make_float2(dt[0] * ex2_ftz(top - gt[0]), dt[1] * ex2_ftz(top - gt[1]));
-        *reinterpret_cast<float2*>(tb + G_V + 2 * lane) =
-            make_float2(dt[0] * ex2_ftz(first - gt[0]), dt[1] * ex2_ftz(first - gt[1]));
-        *reinterpret_cast<float2*>(tb + G_W + 2 * lane) = make_float2(dt[0] * ex2_ftz(rest[0]), dt[1] * ex2_ftz(rest[1]));
-        const float nan = __int_as_float(0x7fc00000);
-        *reinterpret_cast<float2*>(tb + G_EG + 2 * lane) =
-            make_float2(2 * lane >= fb ? nan : ex2_ftz(gt[0]), 2 * lane + 1 >= fb ? nan : ex2_ftz(gt[1]));
+        auto put = [&](int table, const float (&x)[2]) {
+          *reinterpret_cast<float2*>(tb + table + 2 * lane) = make_float2(x[0], x[1]);
+        };
+        put(G_W, w);
+        if constexpr (!STATE_ONLY) {
+          put(G_GAM, high);
+          put(G_LOW, low);
+          put(G_DT, dt);
+          put(G_U, u);
+          put(G_V, v);
+          put(G_EG, eg);
+        }
         if (lane == 0) {
-          decs[buf * 2 + gh] = fb < 64 ? nan : ex2_ftz(g63);
-          steep[buf * 2 + gh] = (far & 1u) | (far >> 7 & 2u) | (far >> 14 & 4u) | (far >> 21 & 8u);
+          decs[buf * 2 + gh] = fb < 64 ? __int_as_float(0x7fc00000) : ex2_ftz(total);
+          if (!STATE_ONLY) steep[buf * 2 + gh] = (far & 1u) | (far >> 7 & 2u) | (far >> 14 & 4u) | (far >> 21 & 8u);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[B_X + buf]);

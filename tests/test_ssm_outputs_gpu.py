@@ -156,3 +156,24 @@ def test_values_that_are_not_finite_in_a_cut_sequence(what):
             y[j, 2:] = True
         assert torch.equal(got[~y], want[~y]) and torch.equal(got_s[~s], want_s[~s])
         assert not got[y].isfinite().any() and not got_s[s].isfinite().any()
+
+
+@pytest.mark.parametrize("P", [64, 128])
+@pytest.mark.parametrize("lens", [[64, 40], [200, 333], [1900]])
+def test_resets_between_weak_decays(P, lens):
+    """Tokens that end a head's memory between tokens that keep it: decays of e^-96 and e^-0.005 within a chunk.  What
+    the weak ones leave is a difference of sums that the strong ones have made large."""
+    T, H = sum(lens), 4
+    m = make((T,), H, P, 2, 128, seed=26)
+    g = torch.Generator(device="cuda").manual_seed(27)
+    strong = torch.rand(T, H, generator=g, device="cuda") < 0.3
+    m["a"] = torch.where(strong, 6.0, -8.0).to(torch.bfloat16)
+    m["A_log"] = torch.full((H,), 2.7726, device="cuda")
+    m["dt_bias"] = torch.zeros(H, device="cuda")
+    m["x"] = torch.where(strong[..., None], 2.0 ** -10 * m["x"], 4 * m["x"])
+    st = torch.randn(len(lens), H, P, 128, device="cuda")
+    out, new = run(m, lens, st)
+    y, ya, S, Sa = reference(m, lens, st)
+    rounded_once(out, y, out_slack(ya, 64))
+    for i in range(len(lens)):
+        L.within(new[i], S[i], (8 * 64 + 200) * 2.0 ** -24 * Sa[i])
