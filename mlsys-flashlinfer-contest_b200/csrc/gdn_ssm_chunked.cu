@@ -138,7 +138,7 @@ enum : int {
   B_STATE,  // the initial state landed
   kNumBars
 };
-static_assert(kNumBars * 8 + 12 <= 256, "barrier area");
+static_assert(kNumBars * 8 + 8 <= 256, "barrier area");
 
 struct Params {
   const float* state;
@@ -356,8 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* first_bad = reinterpret_cast<int*>(smem + L::OFF_BAD);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
-  volatile uint32_t* abort_flag = tmem_slot + 1;
-  volatile uint32_t* any_bad = tmem_slot + 2;
+  volatile uint32_t* any_bad = tmem_slot + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = static_cast<int>(blockIdx.x % p.tiles);
@@ -439,7 +438,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                          : (i == B_RDY_S || i == B_RDY_D || (i >= B_DONE && i < B_DONE + kStages)) ? kComputeWarps
                          : i >= B_X && i < B_EMPTY ? 1 + kHeads : 1);
     fence_mbar_init();
-    *abort_flag = 0u;
     *any_bad = 0u;
     if (state_in) {
       mbar_arrive_expect_tx(&bars[B_STATE], NS / 32 * (kHeads == 2 && !two ? 8192u : 16384u));
@@ -512,9 +510,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&bars[b]);
     };
     // After a timeout a lane waits for nothing any more (its results are garbage, the status word
-    // says so), and its warp leaves the loop.  A test may answer the lanes differently, and the
-    // tensor-memory instructions behind it are the whole warp's: they meet first.  (2 % of the
-    // kernel's time; votes on the test instead were 3 %.)
+    // says so), and its warp leaves the loop; the warps that waited for it time out in turn.  A test may
+    // answer the lanes differently, and the tensor-memory instructions behind it are the whole warp's: they
+    // meet first.  A wait costs ~200 cycles of a chunk's ~4700 even when nothing is left to wait for, so the
+    // warps make none that another covers: a commit stands for every product issued before it.  (Six
+    // waits a chunk instead of four to five, and a flag for timeouts read every chunk: 2-10 %.)
     auto wait = [&](int b, uint32_t parity) {
       if (!failed && !mbar_test(&bars[b], parity)) failed = !wait_long(&bars[b], parity);
       __syncwarp();
@@ -596,6 +596,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     constexpr int kDsBufs = STATE_ONLY ? 2 : 1;
     auto wait_ds = [&](int c) { wait(B_DS + c % kDsBufs, static_cast<uint32_t>((c / kDsBufs) & 1)); };
+    auto wait_last = [&](int c) {  // every product of chunk c
+      if (STATE_ONLY)
+        wait_ds(c);
+      else
+        wait(B_QS, static_cast<uint32_t>(c & 1));
+    };
 
     // ---- W of chunk c by quarters 0-1, in 16-byte pieces of x: a warp takes two tokens at a
     //      time (a token on 16 lanes), four times, 16 tokens apart.  (STATE_ONLY: every warp, twice,
@@ -747,8 +753,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto make_m = [&](int c, int st, uint32_t st_par) {
       wait(B_X + st, st_par);  // (the tables)
-      if (c > 0) wait(B_PV, static_cast<uint32_t>((c - 1) & 1));  // M is free
-      wait(B_G, static_cast<uint32_t>(c & 1));
+      // M is free, and G of this chunk, issued before, is there (a commit covers all products before it)
+      if (c > 0)
+        wait(B_PV, static_cast<uint32_t>((c - 1) & 1));
+      else
+        wait(B_G, 0);
       if (kHeads == 2) {
         if (quarter == 2) {
           m_block(std::false_type{}, cq & 1, cq >> 1, st);
@@ -775,8 +784,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto outputs = [&](int c, int st) {
       float eg[16], qs[16], pv[16];
       load16(table(st, hh) + G_EG + 16 * cq, eg);
-      if (!has_m || c + 1 == n) wait(B_PV, static_cast<uint32_t>(c & 1));  // (the others waited for it to write M)
-      if (c + 1 == n) wait(B_QS, static_cast<uint32_t>(c & 1));  // (before that, the state's update waited for it)
       const bool bad = *any_bad != 0u;  // (written before this chunk's W was signalled)
       tmem_ld16(tl + TM_PV + 64 * hh + 16 * cq, pv);
       tmem_ld16(tl + TM_QS + 16 * cq, qs);
@@ -829,8 +836,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto update = [&](int c, int st) {
       const float dec = decs[st * 2 + hh];
       dprod *= dec;
-      if (c + 1 == n || !has_w)  // (the others waited for it to write W)
-        wait_ds(c);
+      // W^T B is there: the warps that wrote W or M of the next chunk waited for it, or for M X, which comes
+      // after it; the others wait for C S, the chunk's last product
+      const bool met = c + 1 < n && (has_w || has_m);
+      if (!met) wait_last(c);
       float v[kCols];
       if constexpr (kCols == 32)
         tmem_ld32(tl + TM_DS + 128 * (c % kDsBufs) + 32 * cq, v);
@@ -848,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         s[i + 1] = r.y;
       }
       if (!STATE_ONLY && c + 1 < n) {
-        wait(B_QS, static_cast<uint32_t>(c & 1));  // the product that reads the last published state is done
+        if (met) wait_last(c);  // the product that reads the last published state is done
         publish_state();
         if (kHeads == 1) signal(B_RDY_S, false);
       }
@@ -858,8 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int st = 0, prev = 0;
     uint32_t st_par = 0;
     for (int c = -1; c < n; ++c) {
-      if (__any_sync(0xffffffffu, failed || *abort_flag != 0u)) {
-        *abort_flag = 1u;
+      if (__any_sync(0xffffffffu, failed)) {
         failed = true;
         break;
       }
@@ -937,7 +945,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t d = sdesc_sw128_f(bc + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16, 16, 1024);
         mma_ss_by(leader, tm + TM_G, d, d, idesc_g, ks > 0);
       }
-      commit_by(leader, &bars[B_G]);
       return true;
     };
     auto mma_ds = [&](int c, int bst) {
@@ -970,6 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit_by(leader, &bars[B_QS]);
     };
     bool ok = STATE_ONLY || mma_g(0, 0);
+    if (!STATE_ONLY) commit_by(leader, &bars[B_G]);  // (later ones are covered by the commits behind them)
     // stages of chunk c + 1 (of B and C, of x) and of chunk c + 2 (of B and C, with its parity)
     int b1 = 0, x1 = 0, b2 = 1;
     uint32_t par1 = 0, par2 = 0;
