@@ -358,6 +358,9 @@ int gdn_conv_pool(const void *x, int64_t x_batch_stride, int64_t x_row_stride, c
  *   new_state [N, H, P, Ns] fp32
  * output, new_state and workspace may not overlap an input or one another.
  * P (head_dim) and Ns (state_dim) are 64 or 128; num_heads is a multiple of num_groups.
+ * output is off by its rounding to bf16 and 2^-16 of the sums' terms (prompts of more than 16 tokens
+ * a sequence on average; others, and gdn_ssm_pool, sum in fp32: the same tokens may give other bits),
+ * new_state by fp32 arithmetic.
  * The state is in the k-last layout of gdn_prefill.  A sequence of length 0 keeps its
  * state.  Rows of no sequence are left as they were.  Buffers need 16-byte alignment.
  * workspace: gdn_ssm_workspace_bytes bytes, 256-byte aligned (may be NULL when that

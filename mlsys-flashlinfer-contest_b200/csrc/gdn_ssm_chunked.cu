@@ -15,8 +15,8 @@
 // outputs' error was 1.4 times that of their rounding, and the skip factor itself was rounded).  The state
 // itself stays fp32 in registers for the whole piece, and W enters its update as three bf16 terms (24
 // bits of mantissa; B is bf16 already): the final state is as exact as fp32 sums make it.  Two terms left
-// 2.6e-6 of it.  The second terms cost 0-9 % of the time (one prompt of 8192 tokens, 64 heads of 64: 134
-// -> 136 us; four of 8192 327 -> 353; 16 ragged ones, heads of 128: 107 -> 109).
+// 2.6e-6 of it.  The second terms cost about a tenth of the time (four prompts of 8192 tokens, 64 heads of
+// 64: 330 -> 365 us).
 //
 // The decays between a row and the columns of a 16-column block are r_i u_j.  Below the
 // diagonal u_j = dt_j e^{gamma_top - gamma_j} (a table, top = the block's last column) and
@@ -40,12 +40,12 @@
 // columns), warp 16 issues the MMAs, warp 17 the TMA loads and stores, warps 18-19 compute the
 // gate tables of a head each.  The compute warps run, for chunk c: the operands W (quarters
 // 0-1) and M (quarters 2-3) of chunk c + 1, the state update of chunk c, the outputs of
-// chunk c, which go where the chunk's x was and leave by TMA.  Each step's products were issued a
-// step earlier, so no step waits for one to run, and warps meet through mbarriers only (they may
-// be in different steps).  What bounds the kernel is the compute warps' arithmetic and their
-// shared-memory accesses (issue slots ~50 % busy with 4.5 warps a scheduler), not HBM (29 %) or
-// the tensor pipe (30 %): 4 x 16384 tokens, 64 heads of 64, Ns 128: 641 us, 2.5 us a chunk;
-// with neither W nor M formed it would be 1.6 us.
+// chunk c, which go where the chunk's x was and leave by TMA.  Warps meet through mbarriers only (they
+// may be in different steps).  What bounds the kernel is the compute warps' instructions, at five warps a
+// scheduler, and the order in which they and the products wait for one another; counted on 16384 tokens, 64
+// heads of 64, Ns 128 (195 us): 10900 warp instructions a chunk, issue slots 56 % busy, the tensor pipe 34 %,
+// 2200 shared-memory wavefronts a chunk (44 % of the pipe), HBM 20 %.  A chunk of the 4 x 16384 tokens takes 2.7 us
+// (692 us); 128 CTAs run there, one an SM, and 20 SMs have none.
 //
 // Few (sequence, head tile) pairs: sequences are cut into pieces of `seg` tokens.  A first
 // launch (STATE_ONLY) finds each piece's final state from zero and its decay; the second runs

@@ -52,7 +52,10 @@ def run(x, B, C, state, A_log, a, dt_bias, D, cu_seqlens, output=None, new_state
     None (zeros); A_log, dt_bias [H] fp32; D [H] fp32 or None (no skip term);
     cu_seqlens [N+1] int64 (int32 is widened).  Rows of no sequence are left as they
     were in a given ``output``, which may not overlap an input; a sequence of length 0
-    keeps its state."""
+    keeps its state.  Outputs are off by their rounding and 2^-16 of the sums' terms
+    (tensor-core products of two bf16 terms; up to 16 tokens a sequence on average, and
+    ``run_pool``: fp32 sums, so that the same tokens may give other bits), states by
+    fp32 arithmetic."""
     cu_seqlens = _widen(cu_seqlens)
     ext = N.torch_ext()
     if ext is not None:
