@@ -177,3 +177,30 @@ def test_resets_between_weak_decays(P, lens):
     rounded_once(out, y, out_slack(ya, 64))
     for i in range(len(lens)):
         L.within(new[i], S[i], (8 * 64 + 200) * 2.0 ** -24 * Sa[i])
+
+
+def weak_decays(T, bias):
+    """Decays of 1 - 3e-4 and 1 - 2e-3: a state that remembers thousands of tokens."""
+    H, P, Ns = 4, 64, 64
+    m = make((T,), H, P, 1, Ns, seed=28, skip=False)
+    m["a"] = (0.5 * m["a"].float()).to(torch.bfloat16)
+    m["A_log"], m["dt_bias"] = torch.zeros(H, device="cuda"), torch.full((H,), bias, device="cuda")
+    st = torch.randn(1, H, P, Ns, device="cuda")
+    S = st[0].double()
+    dt = torch.nn.functional.softplus(m["a"].double() + bias, threshold=1e9)
+    for t in range(T):
+        S = S * torch.exp(-dt[t])[:, None, None] + (dt[t][:, None] * m["x"][t].double())[..., None] * m["B"][t].double()[:, None]
+    return m, st, S
+
+
+@pytest.mark.parametrize("bias", [-8.0, -6.0])
+def test_long_memory_token_by_token(bias):
+    """Each token's decay is rounded to fp32, to either side: T tokens add up to sqrt(T) 2^-24, 3.3e-6 for 3000.  An
+    exponential that errs to one side adds up to T times that (4.6e-5)."""
+    from gdn_b200 import ssm
+    T = 3000
+    m, st, S = weak_decays(T, bias)
+    pool, slot = st.clone(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    for t0, t1 in ((0, 1000), (1000, 1001), (1001, 1003), (1003, T)):
+        ssm.run_pool(*(m[k][None, t0:t1] for k in ("x", "B", "C")), m["A_log"], m["a"][None, t0:t1], m["dt_bias"], None, pool, slot)
+    assert (pool[0].double() - S).norm() <= 3.3e-6 * S.norm()
