@@ -1094,7 +1094,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           put(G_EG, eg);
         }
         if (lane == 0) {
-          decs[buf * 2 + gh] = fb < 64 ? __int_as_float(0x7fc00000) : ex2_ftz(total);
+          // (rounded to nearest where it is close to 1: the state is multiplied by it once a chunk, and what the
+          // approximation errs to one side would add up)
+          decs[buf * 2 + gh] = fb < 64        ? __int_as_float(0x7fc00000)
+                               : total > -0.7f ? 1.0f + expm1f(total * kLn2)
+                                               : ex2_ftz(total);
           if (!STATE_ONLY) steep[buf * 2 + gh] = (far & 1u) | (far >> 7 & 2u) | (far >> 14 & 4u) | (far >> 21 & 8u);
         }
         __syncwarp();

@@ -204,3 +204,12 @@ def test_long_memory_token_by_token(bias):
     for t0, t1 in ((0, 1000), (1000, 1001), (1001, 1003), (1003, T)):
         ssm.run_pool(*(m[k][None, t0:t1] for k in ("x", "B", "C")), m["A_log"], m["a"][None, t0:t1], m["dt_bias"], None, pool, slot)
     assert (pool[0].double() - S).norm() <= 3.3e-6 * S.norm()
+
+
+@pytest.mark.parametrize("bias", [-8.0, -6.0])
+def test_long_memory_of_a_prompt(bias):
+    """A rounding a chunk: 47 of them, sqrt(47) 2^-24, and the sums' own, a few 2^-24."""
+    T = 3000
+    m, st, S = weak_decays(T, bias)
+    _, new = run(m, [T], st)
+    assert (new[0].double() - S).norm() <= 1e-6 * S.norm()
