@@ -711,26 +711,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         const int md = min(max(mi - r0, -1), 16) + 1;  // row of the mask and skip tables
-        float skip[16];
-        load16(reinterpret_cast<const float*>(smem + L::OFF_SKIP + head * L::kSkipHead + md * L::kSkipPitch), skip);
         float2 q[8];
+        float u[16], rr = r;
         if (!far) {
-          float u[16];
           load16(tb + G_V + r0, u);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            q[k] = __ffma2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
-                              make_float2(r, r), make_float2(skip[2 * k], skip[2 * k + 1]));
         } else {
           const float gi = tb[G_GAM + mi], li = tb[G_LOW + mi];
-          auto decay = [&](int j) { return ex2_ftz(fminf((gi - tb[G_GAM + j]) + (li - tb[G_LOW + j]), 0.f)) * tb[G_DT + j]; };
+          rr = 1.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int j = r0 + 2 * k;
-            q[k].x = fmaf(v[2 * k], decay(j), skip[2 * k]);
-            q[k].y = fmaf(v[2 * k + 1], decay(j + 1), skip[2 * k + 1]);
+          for (int k = 0; k < 16; ++k) {
+            const int j = r0 + k;
+            u[k] = ex2_ftz(fminf((gi - tb[G_GAM + j]) + (li - tb[G_LOW + j]), 0.f)) * tb[G_DT + j];
           }
         }
+        float skip[16];
+        load16(reinterpret_cast<const float*>(smem + L::OFF_SKIP + head * L::kSkipHead + md * L::kSkipPitch), skip);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          q[k] = __ffma2_rn(__fmul2_rn(make_float2(v[2 * k], v[2 * k + 1]), make_float2(u[2 * k], u[2 * k + 1])),
+                            make_float2(rr, rr), make_float2(skip[2 * k], skip[2 * k + 1]));
         const uint4* mask = reinterpret_cast<const uint4*>(smem + L::OFF_MASK + md * L::kMaskPitch);
 #pragma unroll
         for (int k4 = 0; k4 < 2; ++k4) {
